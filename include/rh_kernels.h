@@ -198,6 +198,78 @@ int rh_bias_rope_kv_fp8(void* q, void* k_out_or_null, const void* k_in, const vo
                         uint8_t* k_cache, float* k_scale, uint8_t* v_cache, float* v_scale, const int* at_pos,
                         int seq_len, int num_q_heads, int num_kv_heads, int head_dim, void* stream);
 
+/* ---- A batch of sequences in a paged FP8 cache ----------------------------------------------
+ *
+ * The reference's cache holds one sequence (include/runtherder/engine/kv_cache.h:18-22); these entry points have
+ * no counterpart there.  They serve a batch: sequences share a pool of pages, a table row lists the pages of one
+ * sequence, and everything that changes from step to step is device-resident, so a whole step can be recorded
+ * into a CUDA graph.
+ *
+ * A call names its batch by `rows` (table row of every entry, each at most once; NULL: entry i is row i) and, for
+ * packed tokens, by `cu_seqlens` (num_seqs + 1 non-decreasing offsets: tokens cu_seqlens[i] .. cu_seqlens[i+1]-1
+ * belong to entry i; entries may be empty).  lens[row] is the number of tokens a row holds BEFORE the step, -1 for
+ * an idle row; rh_kv_pages_advance adds the step's tokens at its end.  A step is: reserve; per layer append and
+ * attention; advance.  Rows, lengths and pages are checked where they are used: a token of an idle or unknown row,
+ * or one whose page is missing (-1) or no page of the pool, is not stored, and such a page's keys are not attended.
+ *
+ * `scratch` serves the page operations (reserve, fork, compact); calls on one cache that may overlap in time (two
+ * streams, two graphs) must be ordered by the caller.  The struct is read during the call only. */
+typedef struct rh_kv_pages {
+    uint8_t* k;          /* [num_layers][num_pages][num_kv_heads][page_size][head_dim] E4M3 */
+    uint8_t* v;          /* the same */
+    float* k_scale;      /* [num_layers][num_pages][num_kv_heads][page_size] */
+    float* v_scale;
+    int32_t* page_table; /* [num_rows][pages_per_row], -1: no page */
+    int32_t* lens;       /* [num_rows] tokens held, -1: idle */
+    int32_t* ref_counts; /* [num_pages] rows that list the page, 0: free */
+    int32_t* status;     /* [2], only ever added to: pages that could not be provided; entries refused (a row or page out
+                            of range, a row named twice) */
+    int32_t* scratch;    /* rh_kv_pages_scratch_ints(num_rows, num_pages, pages_per_row) ints */
+    int num_layers;
+    int num_pages;
+    int page_size;       /* a power of two, 16..256 */
+    int num_kv_heads;
+    int head_dim;        /* 64 or 128 */
+    int num_rows;
+    int pages_per_row;
+} rh_kv_pages;
+
+size_t rh_kv_pages_scratch_ints(int num_rows, int num_pages, int pages_per_row);
+
+/* Quantises the new keys and values of a packed batch (bf16 [num_tokens][num_kv_heads][head_dim], k_stride and
+ * v_stride elements between tokens) as rh_quantize_kv_fp8 does and stores them at positions lens[row] + i of
+ * their rows.  Tokens at or behind cu_seqlens[num_seqs] are padding and are not stored. */
+int rh_kv_append_paged_fp8(const rh_kv_pages* cache, int layer, const void* k, const void* v, long long k_stride,
+                           long long v_stride, const int* rows_or_null, const int* cu_seqlens, int num_tokens,
+                           int num_seqs, void* stream);
+
+/* Gives every active row of the batch the pages for its new tokens.  Free pages are handed out lowest first, in
+ * the order of the batch; where they run out the places stay -1 and status[0] counts what is missing. */
+int rh_kv_pages_reserve(const rh_kv_pages* cache, const int* rows_or_null, const int* cu_seqlens, int num_seqs,
+                        void* stream);
+
+/* Drops the pages of `num_rows` rows; their length becomes new_len: 0 (a new, empty sequence) or -1 (idle). */
+int rh_kv_pages_release(const rh_kv_pages* cache, const int* rows_or_null, int num_rows, int new_len, void* stream);
+
+/* lens[row] += the batch's new tokens, for active rows. */
+int rh_kv_pages_advance(const rh_kv_pages* cache, const int* rows_or_null, const int* cu_seqlens, int num_seqs,
+                        void* stream);
+
+/* Row children[i] becomes a copy of row parents[i], all layers: the parent's whole pages are shared, the filled
+ * part of its last page is copied into a free page.  All parents are read before any child is written, so a beam
+ * step may permute rows in one call; what the children held is dropped last.  Of entries that name the same child
+ * the first counts; a child that is its own parent stays as it is; where no page is left for the last part the
+ * child holds the whole pages alone (status[0] counts it). */
+int rh_kv_pages_fork(const rh_kv_pages* cache, const int* parents, const int* children, int count, void* stream);
+
+/* Page dst[i] := page src[i], all layers, codes and scales; tables and counts are left alone.  A page that is a
+ * destination must not be named a second time in the call; pairs with an unknown page are skipped and counted. */
+int rh_kv_pages_copy(const rh_kv_pages* cache, const int* src, const int* dst, int count, void* stream);
+
+/* Packs the used pages to the front of the pool, all layers: the k-th used page at or above the number of used
+ * pages moves to the k-th free page below it, and the page table and the counts follow. */
+int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
+
 /* ---- Decode-loop glue on the device ------------------------------------------------------- */
 
 /* positions[i] = start_pos + i for i < n, *decode_pos = start_pos: what LlamaModel::stage

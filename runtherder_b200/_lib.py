@@ -41,6 +41,14 @@ SIGNATURES = {
     "rh_swiglu_quant_int8": [_p, _p, _p, _p, _p, _i, _i, _p],
     "rh_rope_kv_fp8": [_p, _p, _p, _p, _p, _p, _f, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     "rh_bias_rope_kv_fp8": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    "rh_kv_pages_scratch_ints": [_i, _i, _i],
+    "rh_kv_append_paged_fp8": [_p, _i, _p, _p, _ll, _ll, _p, _p, _i, _i, _p],
+    "rh_kv_pages_reserve": [_p, _p, _p, _i, _p],
+    "rh_kv_pages_release": [_p, _p, _i, _i, _p],
+    "rh_kv_pages_advance": [_p, _p, _p, _i, _p],
+    "rh_kv_pages_fork": [_p, _p, _p, _i, _p],
+    "rh_kv_pages_copy": [_p, _p, _p, _i, _p],
+    "rh_kv_pages_compact": [_p, _p],
     "rh_stage_positions": [_p, _p, _i, _i, _p],
     "rh_decode_advance": [_p, _p, _p, _p, _i, _p],
     "rh_rope_inv_freq_plain": [_p, _i, _f],
@@ -56,7 +64,14 @@ SIGNATURES = {
     "rh_selftest_static": [_p, _i, _p],
 }
 _RESTYPES = {"rh_status_string": C.c_char_p, "rh_last_error_string": C.c_char_p,
-             "rh_flash_split_scratch_floats": C.c_size_t}
+             "rh_flash_split_scratch_floats": C.c_size_t, "rh_kv_pages_scratch_ints": C.c_size_t}
+
+
+class KVPages(C.Structure):
+    """rh_kv_pages of include/rh_kernels.h: the arrays and sizes of a paged cache."""
+
+    _fields_ = [(n, _p) for n in ("k", "v", "k_scale", "v_scale", "page_table", "lens", "ref_counts", "status", "scratch")] + \
+               [(n, _i) for n in ("num_layers", "num_pages", "page_size", "num_kv_heads", "head_dim", "num_rows", "pages_per_row")]
 
 
 class RhError(RuntimeError):

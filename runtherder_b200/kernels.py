@@ -21,7 +21,8 @@ __all__ = [
     "dequantize_w8a8", "quantize_kv_fp8", "dequantize_kv_fp8", "swiglu_bf16_forward", "rope_bf16",
     "embedding_lookup_bf16_forward", "qkv_bias_add_bf16_forward", "stage_positions", "decode_advance",
     "flash_split_scratch_floats", "flash_decode_split_bf16", "flash_prefill_bf16", "tune", "bias_rope_kv_fp8", "rmsnorm_add_quant_int8", "swiglu_quant_int8", "rope_kv_fp8",
-    "rmsnorm_add_last_row", "init",
+    "rmsnorm_add_last_row", "init", "kv_append_paged_fp8", "kv_pages_reserve", "kv_pages_release", "kv_pages_advance",
+    "kv_pages_fork", "kv_pages_copy", "kv_pages_compact",
 ]
 
 
@@ -248,3 +249,75 @@ def bias_rope_kv_fp8(q, k_out, k_in, v_in, q_bias, k_bias, v_bias, positions, in
          _fp8_ptr(k_cache, None, "k_cache"), _ptr(k_scale, _F32, None, "k_scale"),
          _fp8_ptr(v_cache, None, "v_cache"), _ptr(v_scale, _F32, None, "v_scale"), _ptr(at_pos, _I32, 1, "at_pos"),
          seq_len, num_q_heads, num_kv_heads, head_dim, _stream(stream))
+
+
+# ---- a batch of sequences in a paged cache (runtherder_b200.kv_cache.PagedKVCache) -----------------
+
+def _token_rows(t, num_tokens: int, heads: int, head_dim: int, name: str):
+    """Address and token stride of [num_tokens, heads, head_dim] bf16 whose tokens may lie apart (a slice of a
+    fused projection); within a token the values are contiguous."""
+    if isinstance(t, int):
+        return t, heads * head_dim
+    if not t.is_cuda:
+        raise RhError(name, 1, f"{name} must be a CUDA tensor")
+    if t.dtype != _BF:
+        raise RhError(name, 1, f"{name} must have dtype {_BF}, got {t.dtype}")
+    width = heads * head_dim
+    if t.is_contiguous():
+        if t.numel() < num_tokens * width:
+            raise RhError(name, 1, f"{name} holds {t.numel()} elements, {num_tokens * width} needed")
+        return t.data_ptr(), width
+    inside = (head_dim, 1) if t.dim() == 3 else (1,)
+    if t.dim() not in (2, 3) or t.shape[0] < num_tokens or t.stride()[1:] != inside or t.shape[1:].numel() != width or \
+            (t.dim() == 3 and t.shape[2] != head_dim):
+        raise RhError(name, 1, f"{name} must be [tokens, heads, head_dim] with contiguous tokens, got {tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr(), t.stride(0)
+
+
+def _paged_call(cache, fn: str, *args) -> None:
+    """An entry point on a paged cache, on the cache's device."""
+    if cache.device_index != torch.cuda.current_device():
+        raise RhError(fn, 1, f"the cache is on device {cache.device_index}, the current device is {torch.cuda.current_device()}")
+    call(fn, cache.desc, *args)
+
+
+def kv_append_paged_fp8(cache, layer: int, k, v, cu_seqlens, num_tokens: int, num_seqs: int, rows=None, stream=None) -> None:
+    """Quantises the packed batch's new keys and values [num_tokens, Hkv, D] into its rows' pages, at positions lens[row]
+    and on.  Tokens at or behind cu_seqlens[num_seqs] are padding."""
+    kp, ks = _token_rows(k, num_tokens, cache.num_kv_heads, cache.head_dim, "k")
+    vp, vs = _token_rows(v, num_tokens, cache.num_kv_heads, cache.head_dim, "v")
+    _paged_call(cache, "rh_kv_append_paged_fp8", layer, kp, vp, ks, vs, _ptr(rows, _I32, num_seqs, "rows"),
+                _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, _stream(stream))
+
+
+def kv_pages_reserve(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
+    """Gives the batch's active rows the pages that their new tokens need: the lowest free ones, in the order of the batch."""
+    _paged_call(cache, "rh_kv_pages_reserve", _ptr(rows, _I32, num_seqs, "rows"), _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
+                num_seqs, _stream(stream))
+
+
+def kv_pages_release(cache, num_rows: int, rows=None, new_len: int = -1, stream=None) -> None:
+    """Drops the rows' pages; new_len 0 starts an empty sequence, -1 leaves the row idle."""
+    _paged_call(cache, "rh_kv_pages_release", _ptr(rows, _I32, num_rows, "rows"), num_rows, new_len, _stream(stream))
+
+
+def kv_pages_advance(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
+    """lens[row] += the batch's new tokens, at the end of a step."""
+    _paged_call(cache, "rh_kv_pages_advance", _ptr(rows, _I32, num_seqs, "rows"), _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
+                num_seqs, _stream(stream))
+
+
+def kv_pages_fork(cache, parents, children, count: int, stream=None) -> None:
+    """Row children[i] becomes a copy of row parents[i]: whole pages are shared, the filled part of the last one is copied."""
+    _paged_call(cache, "rh_kv_pages_fork", _ptr(parents, _I32, count, "parents"), _ptr(children, _I32, count, "children"), count,
+                _stream(stream))
+
+
+def kv_pages_copy(cache, src, dst, count: int, stream=None) -> None:
+    """Page dst[i] := page src[i] in every layer; the tables are left alone."""
+    _paged_call(cache, "rh_kv_pages_copy", _ptr(src, _I32, count, "src"), _ptr(dst, _I32, count, "dst"), count, _stream(stream))
+
+
+def kv_pages_compact(cache, stream=None) -> None:
+    """Packs the used pages to the front of the pool; the page table and the reference counts follow."""
+    _paged_call(cache, "rh_kv_pages_compact", _stream(stream))
