@@ -270,6 +270,23 @@ int rh_kv_pages_copy(const rh_kv_pages* cache, const int* src, const int* dst, i
  * pages moves to the k-th free page below it, and the page table and the counts follow. */
 int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
 
+/* Attention of one new token per batch entry: out[b,h,:] = softmax_j(scale * q[b,h] . K[j]) V[j] over the keys
+ * j = 0 .. lens[row of b] of its row (as rh_flash_decode_split_bf16: the new token's key sits at lens[row], appended
+ * before this call).  out [num_seqs][num_q_heads][head_dim] bf16; q the same with q_stride elements between entries.
+ * An entry whose row is idle, or that sees no key, gets zeros.  Several entries may name the same row here.
+ *
+ * shared_pages / shared_len (both or neither; device memory): the first *shared_len keys of every active entry lie in
+ * the pages shared_pages[0], shared_pages[1], ... (e.g. the page-table row of any entry after rh_kv_pages_fork), and
+ * these are read once for all entries.  An entry that holds fewer keys attends those it holds.  The entries' own
+ * table rows list the shared pages too; what is shared beyond a multiple of 256 keys is read through them.
+ *
+ * partial: caller-owned scratch of rh_flash_decode_paged_scratch_floats(...) floats, 16-byte aligned; calls that may
+ * overlap in time need one each.  num_seqs <= 4096.  Two kernels; results do not depend on timing. */
+size_t rh_flash_decode_paged_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
+int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_stride, const rh_kv_pages* cache, int layer,
+                               const int* rows_or_null, int num_seqs, int num_q_heads, float scale, float* partial,
+                               const int* shared_pages_or_null, const int* shared_len_or_null, void* stream);
+
 /* ---- Decode-loop glue on the device ------------------------------------------------------- */
 
 /* positions[i] = start_pos + i for i < n, *decode_pos = start_pos: what LlamaModel::stage

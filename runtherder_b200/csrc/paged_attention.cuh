@@ -1,0 +1,84 @@
+// What the attention kernels on the paged cache share: the arguments of a decode step, the layout of its scratch, and
+// the constants of the softmax states they exchange.
+//
+// A state of a query row over some of its keys is (m, l, acc[D]) with out = acc / l over those keys; m is a log2-domain
+// exponent to which l and acc are relative, so states over disjoint keys add up as 2^(m - M) (l, acc).
+#pragma once
+#include <climits>
+
+#include "paged.cuh"
+
+namespace rh {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMInit = -1.0e30f;    // m before any key (finite: differences stay defined)
+constexpr float kLgFloor = -100.0f;   // floor of log2(V scale): a zero scale must not give -inf - -inf
+constexpr int kMaxSeqs = 4096;        // sequences of a decode call
+constexpr int kOwnCols = 8;           // query heads of a segment of own keys
+constexpr int kPrefixCols = 16;       // query rows of a prefix segment
+constexpr int kHeaderInts = 4;        // {shared keys, own tiles per head, -, -}, then the first tile of every sequence
+constexpr int kSharedAlign = 256;     // the prefix is cut down to a multiple of this (the largest page), the rest is own
+
+struct DecodeArgs {
+    Layer c;
+    __nv_bfloat16* out;
+    const __nv_bfloat16* q;
+    long long q_stride;        // elements between sequences
+    const int* rows;
+    const int* shared_pages;   // null: nothing is shared
+    const int* shared_len;
+    int* header;
+    float* own_states;
+    float* prefix_states;
+    float* block_ml;           // [splits][rows][2] and [splits][rows][D], where the tensor-memory kernel takes the prefix
+    float* block_acc;
+    int* error_word;
+    int num_seqs;
+    int group;                 // query heads per kv head
+    int head_chunks;
+    int own_cols;
+    int prefix_chunks;         // 0: nothing is shared, or the tensor-memory kernel takes it
+    int block_splits;
+    float scale_log2e;
+
+    __device__ __forceinline__ int shared_keys() const {
+        if (shared_len == nullptr) return 0;
+        const int room = c.pages_per_row << c.page_shift;
+        const int n = min(*shared_len, room);
+        return n < kSharedAlign ? 0 : n - n % kSharedAlign;
+    }
+};
+
+// States of `cols` query rows: m [cols], l [cols], then acc [cols][dim] from a 16-byte boundary on.
+__host__ __device__ constexpr int acc_offset(int cols) { return (2 * cols + 3) / 4 * 4; }
+__host__ __device__ constexpr long long state_floats(int cols, int dim) { return acc_offset(cols) + static_cast<long long>(cols) * dim; }
+
+// Warps of the grid that get tiles: at least kMinTilesPerWarp each where there are enough.
+constexpr int kMinTilesPerWarp = 2;
+__device__ __forceinline__ long long warps_in_use(long long total, long long warps) {
+    const long long most = (total + kMinTilesPerWarp - 1) / kMinTilesPerWarp;
+    return most < 1 ? 1 : (most < warps ? most : warps);
+}
+
+inline int decode_ctas() { return 3 * host::num_sms(); }
+
+struct DecodeScratch {
+    size_t own, prefix, block_ml, block_acc, floats;
+};
+inline DecodeScratch decode_scratch(int num_seqs, int num_q_heads, int num_kv_heads, int dim) {
+    const int group = num_q_heads / num_kv_heads, chunks = (group + kOwnCols - 1) / kOwnCols;
+    const int cols = group < kOwnCols ? group : kOwnCols;
+    const size_t warps = static_cast<size_t>(decode_ctas()) * 4;
+    DecodeScratch s = {};
+    s.own = (static_cast<size_t>(kHeaderInts + num_seqs + 1) + 3) / 4 * 4;
+    s.prefix = s.own + (static_cast<size_t>(num_seqs) * num_kv_heads * chunks + warps) * static_cast<size_t>(state_floats(cols, dim));
+    const size_t prefix_segs = static_cast<size_t>(num_kv_heads) * ((static_cast<size_t>(num_seqs) * group + kPrefixCols - 1) / kPrefixCols);
+    s.block_ml = s.prefix + (num_seqs > 1 ? (prefix_segs + warps) * static_cast<size_t>(state_floats(kPrefixCols, dim)) : 0);
+    s.block_acc = s.block_ml;
+    s.floats = s.block_acc;
+    return s;
+}
+
+}  // namespace paged
+}  // namespace rh

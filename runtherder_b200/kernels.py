@@ -22,7 +22,7 @@ __all__ = [
     "embedding_lookup_bf16_forward", "qkv_bias_add_bf16_forward", "stage_positions", "decode_advance",
     "flash_split_scratch_floats", "flash_decode_split_bf16", "flash_prefill_bf16", "tune", "bias_rope_kv_fp8", "rmsnorm_add_quant_int8", "swiglu_quant_int8", "rope_kv_fp8",
     "rmsnorm_add_last_row", "init", "kv_append_paged_fp8", "kv_pages_reserve", "kv_pages_release", "kv_pages_advance",
-    "kv_pages_fork", "kv_pages_copy", "kv_pages_compact",
+    "kv_pages_fork", "kv_pages_copy", "kv_pages_compact", "flash_decode_paged_bf16", "flash_decode_paged_scratch_floats",
 ]
 
 
@@ -274,10 +274,14 @@ def _token_rows(t, num_tokens: int, heads: int, head_dim: int, name: str):
     return t.data_ptr(), t.stride(0)
 
 
-def _paged_call(cache, fn: str, *args) -> None:
-    """An entry point on a paged cache, on the cache's device."""
+def _on_device(cache, fn: str) -> None:
     if cache.device_index != torch.cuda.current_device():
         raise RhError(fn, 1, f"the cache is on device {cache.device_index}, the current device is {torch.cuda.current_device()}")
+
+
+def _paged_call(cache, fn: str, *args) -> None:
+    """An entry point whose first argument is a paged cache, on the cache's device."""
+    _on_device(cache, fn)
     call(fn, cache.desc, *args)
 
 
@@ -321,3 +325,22 @@ def kv_pages_copy(cache, src, dst, count: int, stream=None) -> None:
 def kv_pages_compact(cache, stream=None) -> None:
     """Packs the used pages to the front of the pool; the page table and the reference counts follow."""
     _paged_call(cache, "rh_kv_pages_compact", _stream(stream))
+
+
+def flash_decode_paged_scratch_floats(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Floats of scratch that flash_decode_paged_bf16 needs on the current device."""
+    from ._lib import lib
+    return int(lib.rh_flash_decode_paged_scratch_floats(num_seqs, num_q_heads, num_kv_heads, head_dim))
+
+
+def flash_decode_paged_bf16(out, q, cache, layer: int, num_seqs: int, num_q_heads: int, scale: float, partial, shared_pages=None,
+                            shared_len=None, rows=None, stream=None) -> None:
+    """One new token per entry attends keys 0..lens[row] of its row.  shared_pages / shared_len: the first *shared_len keys of
+    every entry lie in these pages (a page-table row) and are read once for all of them."""
+    fn, D = "rh_flash_decode_paged_bf16", cache.head_dim
+    _on_device(cache, fn)
+    qp, qs = _token_rows(q, num_seqs, num_q_heads, D, "q")
+    need = flash_decode_paged_scratch_floats(num_seqs, num_q_heads, cache.num_kv_heads, D)
+    call(fn, _ptr(out, _BF, num_seqs * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _ptr(rows, _I32, num_seqs, "rows"), num_seqs,
+         num_q_heads, float(scale), _ptr(partial, _F32, need, "partial"), _ptr(shared_pages, _I32, None, "shared_pages"),
+         _ptr(shared_len, _I32, 1, "shared_len"), _stream(stream))

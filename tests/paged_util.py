@@ -156,3 +156,39 @@ def attend(q, k, v, first, scale):
     vs = torch.where(seen.any(0)[None, :, None], vv, torch.zeros_like(vv))
     o = torch.einsum("hnk,hkd->hnd", e, vs) / torch.where(total > 0, total, torch.ones_like(total))
     return o.permute(1, 0, 2)
+
+
+def check_attention(out, q, k, v, first, scale, what="", weight_step=2.0 ** -11, extra=0.0):
+    """Holds tokens `out` [n, heads, D] (bf16) against attend() in 64 bits, within what the arithmetic allows, derived:
+
+      the store            a bf16 rounding                                                    2^-8 |o|
+      the weights          one f16 rounding each (`weight_step`), on A = sum_j p_j |v_j|      2^-11 A
+      the scores           fp32 sums of exact products: 2^-18 of B = max_j sum_d |q_d k_jd|, and the log2-domain score's own
+                           roundings, three of 2^-23 of its size and the V scale's (at most 40); numerator and
+                           denominator both carry them                                       2 (2^-18 scale B + 2^-21 (|x| + 40)) A
+      small weights        f16 loses weights below 2^-24 in units where the largest is 2^10   n 2^-34 max |v|
+      `extra`              of A, for forms that round once more
+    """
+    n, hq, dim = q.shape
+    want = attend(q, k, v, first, scale)
+    kk, vv = k.repeat_interleave(hq // k.shape[0], 0), v.repeat_interleave(hq // v.shape[0], 0)
+    seen = (torch.arange(kk.shape[1], device=q.device)[None] < (first + torch.arange(n, device=q.device))[:, None])[None]
+    fk, fv = torch.nan_to_num(kk), torch.nan_to_num(vv)
+    z = torch.einsum("nhd,hkd->hnk", q.double(), fk) * scale
+    big = torch.where(seen, torch.einsum("nhd,hkd->hnk", q.double().abs(), fk.abs()), torch.zeros_like(z)).amax(-1, keepdim=True) * scale
+    top = torch.where(seen, z.abs(), torch.zeros_like(z)).amax(-1, keepdim=True) / math.log(2.0)
+    zz = z.masked_fill(~seen, -math.inf)
+    m = zz.amax(-1, keepdim=True)
+    p = torch.exp(zz - torch.where(torch.isinf(m), torch.zeros_like(m), m))
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    a = torch.einsum("hnk,hkd->hnd", p, fv.abs())
+    delta = 2.0 * (2.0 ** -18 * big + 2.0 ** -21 * (top + 40.0))
+    small = kk.shape[1] * 2.0 ** -34 * fv.abs().amax(-2, keepdim=True) if kk.shape[1] else 0.0
+    tol = (2.0 ** -8 * want.abs() + ((weight_step + delta + extra) * a + small).permute(1, 0, 2)) + 1e-30
+    got = out.double()
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), finite), (what, "finite where the exact value is not, or the other way round")
+    err = torch.where(finite, (got - want).abs(), torch.zeros_like(tol))
+    worst = float((err / tol).nan_to_num().max()) if err.numel() else 0.0
+    assert worst <= 1.0, (what, worst)
+    return worst
