@@ -270,6 +270,21 @@ int rh_kv_pages_copy(const rh_kv_pages* cache, const int* src, const int* dst, i
  * pages moves to the k-th free page below it, and the page table and the counts follow. */
 int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
 
+/* Causal attention of a packed batch's new tokens: token i of an entry attends keys 0 .. lens[row] + i of its row
+ * (its keys were appended before this call).  out [num_tokens][num_q_heads][head_dim] bf16; q the same with q_stride
+ * elements between tokens.  Tokens of an idle or unknown row get zeros; tokens at or behind cu_seqlens[num_seqs] are
+ * padding, and their rows of out are left as they were.
+ * num_splits > 1 (long histories in front of few new tokens) deals every row's keys to that many CTAs, whose states are
+ * joined from partial_or_null: scratch of rh_flash_prefill_packed_scratch_floats(...) floats, 16-byte aligned, one per call that
+ * may overlap in time.  rh_flash_prefill_packed_splits suggests a count (max_keys: the longest row with its new tokens).
+ * tcgen05 kernel, one CTA per SM holding 256 or all 512 of its tensor-memory columns for its lifetime. */
+int rh_flash_prefill_packed_splits(int num_tokens, int num_seqs, int max_keys, int num_q_heads, int num_kv_heads,
+                                   int head_dim);
+size_t rh_flash_prefill_packed_scratch_floats(int num_tokens, int num_q_heads, int head_dim, int num_splits);
+int rh_flash_prefill_packed_bf16(void* out, const void* q, long long q_stride, const rh_kv_pages* cache, int layer,
+                                 const int* rows_or_null, const int* cu_seqlens, int num_tokens, int num_seqs,
+                                 int num_q_heads, float scale, float* partial_or_null, int num_splits, void* stream);
+
 /* Attention of one new token per batch entry: out[b,h,:] = softmax_j(scale * q[b,h] . K[j]) V[j] over the keys
  * j = 0 .. lens[row of b] of its row (as rh_flash_decode_split_bf16: the new token's key sits at lens[row], appended
  * before this call).  out [num_seqs][num_q_heads][head_dim] bf16; q the same with q_stride elements between entries.
@@ -281,7 +296,8 @@ int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
  * table rows list the shared pages too; what is shared beyond a multiple of 256 keys is read through them.
  *
  * partial: caller-owned scratch of rh_flash_decode_paged_scratch_floats(...) floats, 16-byte aligned; calls that may
- * overlap in time need one each.  num_seqs <= 4096.  Two kernels; results do not depend on timing. */
+ * overlap in time need one each.  num_seqs <= 4096.  Two kernels, three where the prefix
+ * meets 65 or more query rows per kv head (it then runs on tcgen05); results do not depend on timing. */
 size_t rh_flash_decode_paged_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
 int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_stride, const rh_kv_pages* cache, int layer,
                                const int* rows_or_null, int num_seqs, int num_q_heads, float scale, float* partial,

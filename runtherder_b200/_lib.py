@@ -49,6 +49,9 @@ SIGNATURES = {
     "rh_kv_pages_fork": [_p, _p, _p, _i, _p],
     "rh_kv_pages_copy": [_p, _p, _p, _i, _p],
     "rh_kv_pages_compact": [_p, _p],
+    "rh_flash_prefill_packed_splits": [_i, _i, _i, _i, _i, _i],
+    "rh_flash_prefill_packed_scratch_floats": [_i, _i, _i, _i],
+    "rh_flash_prefill_packed_bf16": [_p, _p, _ll, _p, _i, _p, _p, _i, _i, _i, _f, _p, _i, _p],
     "rh_flash_decode_paged_scratch_floats": [_i, _i, _i, _i],
     "rh_flash_decode_paged_bf16": [_p, _p, _ll, _p, _i, _p, _i, _i, _f, _p, _p, _p, _p],
     "rh_stage_positions": [_p, _p, _i, _i, _p],
@@ -67,7 +70,7 @@ SIGNATURES = {
 }
 _RESTYPES = {"rh_status_string": C.c_char_p, "rh_last_error_string": C.c_char_p,
              "rh_flash_split_scratch_floats": C.c_size_t, "rh_kv_pages_scratch_ints": C.c_size_t,
-             "rh_flash_decode_paged_scratch_floats": C.c_size_t}
+             "rh_flash_decode_paged_scratch_floats": C.c_size_t, "rh_flash_prefill_packed_scratch_floats": C.c_size_t}
 
 
 class KVPages(C.Structure):

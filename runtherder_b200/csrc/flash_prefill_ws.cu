@@ -29,6 +29,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "flash_prefill_roles.cuh"
 #include "flash_prefill_tc.cuh"
 #include "rh_kernels.h"
 
@@ -74,38 +75,6 @@ struct Geo {
 };
 enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
 
-constexpr int kTries = 1 << 20;
-constexpr int kLazyNs = 100;      // pause between polls of the product and conversion warps
-
-// Bounded wait that also ends when another thread of the CTA has given up.  kBackoffNs > 0 sleeps between
-// tries: for the roles whose reaction time is not on the critical path (a poll is a shared-memory access and
-// an issue slot taken from the softmax warps).
-template <int kBackoffNs = 0>
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int where, int* error_word,
-                                           int tries = kTries, int* tries_used = nullptr) {
-    const uint32_t addr = pipe::smem_u32(bar);
-    for (int i = 0; i < tries; ++i) {       // a try blocks for a while in hardware before it reports failure
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (ok != 0) return true;
-        if ((i & 15) == 15 && *gave_up != 0) {                 // looked at now and then: a poll is a shared-memory access
-            if (tries_used != nullptr) *tries_used = i + 1;
-            return false;
-        }
-        if constexpr (kBackoffNs > 0) __nanosleep(kBackoffNs);
-    }
-    *gave_up = 1;
-    if (error_word != nullptr) atomicCAS(error_word, 0, (where << 8) | 1);
-    if (tries_used != nullptr) *tries_used = tries;
-    return false;
-}
-
 // Probe of the give-up path of wait_phase (rh_selfcheck_role_wait): warp 0 waits with a limit of `tries` on a
 // barrier that nothing completes and must give up; warp 1 waits with the kernels' own limit on another such
 // barrier and must be released by warp 0's flag long before that limit.  out: [0] warp 0's wait returned true (0
@@ -132,22 +101,6 @@ __global__ void role_wait_probe_kernel(int tries, int* out) {
     __syncthreads();
     if (threadIdx.x == 0) out[1] = flag[0];
 }
-
-// Barrier among the `count` threads that use named barrier `id`, returning the OR of their predicates.
-__device__ __forceinline__ bool group_or(int id, int count, bool pred) {
-    uint32_t out;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %3, 0;\n\t"
-        "bar.red.or.pred p, %1, %2, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(out)
-        : "r"(id), "r"(count), "r"(static_cast<uint32_t>(pred))
-        : "memory");
-    return out != 0;
-}
-
-// the key whose K row becomes row r of the K operand tile (S column 16a + 8h + 2c + e holds key 16a + 4c + 2h + e)
-__device__ __forceinline__ int key_of_k_row(int r) { return (r & 48) | ((r & 6) << 1) | ((r & 8) >> 2) | (r & 1); }
 
 // grid (token tiles of kBlocks * tokens_per_cta tokens, num_kv_heads * head_chunks)
 template <int kBlocks>

@@ -63,6 +63,10 @@ __device__ __forceinline__ long long warps_in_use(long long total, long long war
 
 inline int decode_ctas() { return 3 * host::num_sms(); }
 
+// Query rows per kv head (entries x group) from which the tensor-memory kernel takes the prefix.
+constexpr int kBlockRows = 65;
+int prefix_splits(int num_seqs, int num_kv_heads, int group);
+
 struct DecodeScratch {
     size_t own, prefix, block_ml, block_acc, floats;
 };
@@ -73,10 +77,18 @@ inline DecodeScratch decode_scratch(int num_seqs, int num_q_heads, int num_kv_he
     DecodeScratch s = {};
     s.own = (static_cast<size_t>(kHeaderInts + num_seqs + 1) + 3) / 4 * 4;
     s.prefix = s.own + (static_cast<size_t>(num_seqs) * num_kv_heads * chunks + warps) * static_cast<size_t>(state_floats(cols, dim));
-    const size_t prefix_segs = static_cast<size_t>(num_kv_heads) * ((static_cast<size_t>(num_seqs) * group + kPrefixCols - 1) / kPrefixCols);
-    s.block_ml = s.prefix + (num_seqs > 1 ? (prefix_segs + warps) * static_cast<size_t>(state_floats(kPrefixCols, dim)) : 0);
-    s.block_acc = s.block_ml;
-    s.floats = s.block_acc;
+    s.block_ml = s.block_acc = s.floats = s.prefix;
+    if (num_seqs == 1) return s;
+    const size_t rows = static_cast<size_t>(num_seqs) * group;
+    if (rows < kBlockRows) {
+        const size_t segs = static_cast<size_t>(num_kv_heads) * ((rows + kPrefixCols - 1) / kPrefixCols);
+        s.floats = s.prefix + (segs + warps) * static_cast<size_t>(state_floats(kPrefixCols, dim));
+    } else {
+        const size_t states = static_cast<size_t>(prefix_splits(num_seqs, num_kv_heads, group)) * num_seqs * num_q_heads;
+        s.block_acc = (s.prefix + 3) / 4 * 4;
+        s.block_ml = s.block_acc + states * dim;
+        s.floats = s.block_ml + states * 2;
+    }
     return s;
 }
 

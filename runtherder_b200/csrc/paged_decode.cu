@@ -27,6 +27,7 @@
 #include "flash_prefill_tc.cuh"
 #include "paged.cuh"
 #include "paged_attention.cuh"
+#include "paged_prefill.cuh"
 #include "rh_kernels.h"
 #include "rh_pipeline.cuh"
 
@@ -636,8 +637,15 @@ extern "C" int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_
     a.header = reinterpret_cast<int*>(partial);
     a.own_states = partial + parts.own;
     a.prefix_states = partial + parts.prefix;
-    if (a.shared_pages != nullptr) a.prefix_chunks = (num_seqs * a.group + paged::kPrefixCols - 1) / paged::kPrefixCols;
+    a.block_ml = partial + parts.block_ml;
+    a.block_acc = partial + parts.block_acc;
+    if (a.shared_pages != nullptr) {
+        if (num_seqs * a.group < paged::kBlockRows) a.prefix_chunks = (num_seqs * a.group + paged::kPrefixCols - 1) / paged::kPrefixCols;
+        else a.block_splits = paged::prefix_splits(num_seqs, cache->num_kv_heads, a.group);
+    }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (const int e = cache->head_dim == 128 ? paged::launch_decode<128>(a, s, fn) : paged::launch_decode<64>(a, s, fn)) return e;
+    if (a.block_splits > 0)
+        if (const int e = paged::launch_prefix(a, cache->head_dim, s, fn)) return e;
     return cache->head_dim == 128 ? paged::launch_join<128>(a, s, fn) : paged::launch_join<64>(a, s, fn);
 }

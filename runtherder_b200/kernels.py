@@ -23,6 +23,7 @@ __all__ = [
     "flash_split_scratch_floats", "flash_decode_split_bf16", "flash_prefill_bf16", "tune", "bias_rope_kv_fp8", "rmsnorm_add_quant_int8", "swiglu_quant_int8", "rope_kv_fp8",
     "rmsnorm_add_last_row", "init", "kv_append_paged_fp8", "kv_pages_reserve", "kv_pages_release", "kv_pages_advance",
     "kv_pages_fork", "kv_pages_copy", "kv_pages_compact", "flash_decode_paged_bf16", "flash_decode_paged_scratch_floats",
+    "flash_prefill_packed_bf16", "flash_prefill_packed_splits", "flash_prefill_packed_scratch_floats",
 ]
 
 
@@ -344,3 +345,28 @@ def flash_decode_paged_bf16(out, q, cache, layer: int, num_seqs: int, num_q_head
     call(fn, _ptr(out, _BF, num_seqs * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _ptr(rows, _I32, num_seqs, "rows"), num_seqs,
          num_q_heads, float(scale), _ptr(partial, _F32, need, "partial"), _ptr(shared_pages, _I32, None, "shared_pages"),
          _ptr(shared_len, _I32, 1, "shared_len"), _stream(stream))
+
+
+def flash_prefill_packed_splits(num_tokens: int, num_seqs: int, max_keys: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Into how many key ranges flash_prefill_packed_bf16 had best deal the keys of this batch (max_keys: its longest row with
+    the new tokens): more than one where few new tokens stand behind long histories."""
+    from ._lib import lib
+    return int(lib.rh_flash_prefill_packed_splits(num_tokens, num_seqs, max_keys, num_q_heads, num_kv_heads, head_dim))
+
+
+def flash_prefill_packed_scratch_floats(num_tokens: int, num_q_heads: int, head_dim: int, num_splits: int) -> int:
+    """Floats of scratch that flash_prefill_packed_bf16 needs for this many key ranges (0 for one)."""
+    from ._lib import lib
+    return int(lib.rh_flash_prefill_packed_scratch_floats(num_tokens, num_q_heads, head_dim, num_splits))
+
+
+def flash_prefill_packed_bf16(out, q, cache, layer: int, cu_seqlens, num_tokens: int, num_seqs: int, num_q_heads: int, scale: float,
+                              partial=None, num_splits: int = 1, rows=None, stream=None) -> None:
+    """A packed batch's new tokens attend causally: token i of an entry sees keys 0..lens[row] + i of its row."""
+    fn, D = "rh_flash_prefill_packed_bf16", cache.head_dim
+    _on_device(cache, fn)
+    qp, qs = _token_rows(q, num_tokens, num_q_heads, D, "q")
+    need = flash_prefill_packed_scratch_floats(num_tokens, num_q_heads, D, num_splits)
+    call(fn, _ptr(out, _BF, num_tokens * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _ptr(rows, _I32, num_seqs, "rows"),
+         _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, num_q_heads, float(scale),
+         _ptr(partial, _F32, need, "partial") if num_splits > 1 else None, num_splits, _stream(stream))

@@ -158,16 +158,20 @@ def attend(q, k, v, first, scale):
     return o.permute(1, 0, 2)
 
 
-def check_attention(out, q, k, v, first, scale, what="", weight_step=2.0 ** -11, extra=0.0):
+def check_attention(out, q, k, v, first, scale, what="", extra=0.0, small_step=2.0 ** -34, mixed=False):
     """Holds tokens `out` [n, heads, D] (bf16) against attend() in 64 bits, within what the arithmetic allows, derived:
 
       the store            a bf16 rounding                                                    2^-8 |o|
-      the weights          one f16 rounding each (`weight_step`), on A = sum_j p_j |v_j|      2^-11 A
+      the weights          one f16 rounding each, on A = sum_j p_j |v_j|                      2^-11 A
       the scores           fp32 sums of exact products: 2^-18 of B = max_j sum_d |q_d k_jd|, and the log2-domain score's own
                            roundings, three of 2^-23 of its size and the V scale's (at most 40); numerator and
                            denominator both carry them                                       2 (2^-18 scale B + 2^-21 (|x| + 40)) A
-      small weights        f16 loses weights below 2^-24 in units where the largest is 2^10   n 2^-34 max |v|
+      small weights        f16 loses what is below 2^-24 in units where the largest is 2^10   n 2^-34 max |v|   (`small_step`: 2^-25
+                           where the largest weight may be 1: half a step of 2^-24)
       `extra`              of A, for forms that round once more
+      `mixed`              keys whose V scale rides in the exponent beside keys whose scale is folded into V, times 2^8: the
+                           latter's weights are taken relative to a maximum that is up to 2^(lg vs + 8) higher, |v| <= 224:
+                           n 2^-25 2^7 max_i p_i max |v_i|
     """
     n, hq, dim = q.shape
     want = attend(q, k, v, first, scale)
@@ -183,8 +187,10 @@ def check_attention(out, q, k, v, first, scale, what="", weight_step=2.0 ** -11,
     p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
     a = torch.einsum("hnk,hkd->hnd", p, fv.abs())
     delta = 2.0 * (2.0 ** -18 * big + 2.0 ** -21 * (top + 40.0))
-    small = kk.shape[1] * 2.0 ** -34 * fv.abs().amax(-2, keepdim=True) if kk.shape[1] else 0.0
-    tol = (2.0 ** -8 * want.abs() + ((weight_step + delta + extra) * a + small).permute(1, 0, 2)) + 1e-30
+    small = kk.shape[1] * small_step * fv.abs().amax((-2, -1), keepdim=True)
+    if mixed:
+        small = small + kk.shape[1] * 2.0 ** -18 * (p * fv.abs().amax(-1)[:, None]).amax(-1, keepdim=True)
+    tol = (2.0 ** -8 * want.abs() + ((2.0 ** -11 + delta + extra) * a + small).permute(1, 0, 2)) + 1e-30
     got = out.double()
     finite = torch.isfinite(want)
     assert torch.equal(torch.isfinite(got), finite), (what, "finite where the exact value is not, or the other way round")
