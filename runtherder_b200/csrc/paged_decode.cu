@@ -165,7 +165,7 @@ struct Walk {
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
-            e = amax > 0.0f ? max(-100, min(100, e)) : 0;
+            e = amax > 0.0f ? max(-100, min(126, e)) : 0;
             const float down = __int_as_float((127 - e) << 23);
             const float mine = p.scale_log2e * __int_as_float((127 + e) << 23);
             factor[nt][0] = __shfl_sync(0xffffffffu, mine, 8 * c);

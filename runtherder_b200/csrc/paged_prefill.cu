@@ -5,28 +5,37 @@
 //   prefix    the shared keys of a decode step: every entry of the batch is one token, all see the same keys
 //
 // The reference's counterpart is flash_prefill_bf16 (include/runtherder/kernels/flash_prefill.cuh:27-40), one sequence
-// in a contiguous cache.  Geometry and roles are those of flash_prefill_ws.cu: a CTA carries one or two blocks of 128
-// query rows of one kv head (the group's heads x consecutive tokens), walks key tiles of 64, S and O in tensor memory
+// in a contiguous cache.  As in flash_prefill_ws.cu a CTA carries one or two blocks of 128 query rows of one kv head (the
+// group's heads x consecutive tokens), walks key tiles of 64, keeps S and O in tensor memory, and splits the work by role:
 //
-//   S[128 x 64] = Q K^T      (f16: bf16 queries, E4M3 keys: both exact in f16)          tcgen05.mma, operands in shared memory
-//   O[128 x D] += W V        W = 2^(S ks - m) as f16 in tensor memory
+//   S[128 x 64] = Q K^T      E4M3 x E4M3 (tcgen05 kind::f8f6f4), operands in shared memory
+//   O[128 x D] += W V        f16 (kind::f16): W = 2^(S c ks - m) in tensor memory, V = code x V scale in shared memory
 //
 //   softmax warps (8 per block)   scores -> weights; two rows x sixteen keys per thread
 //   product warp (1 per block)    issues the products
-//   conversion warps              raw E4M3 tiles -> f16 operand tiles
-//   copy warp                     fetches raw tiles page by page with bulk copies, two tiles ahead
+//   conversion warps (4)          raw E4M3 V tiles -> f16 operand tiles, scales folded in
+//   copy warp                     fetches K tiles (tensor-map copies, swizzled as the product wants them), V tiles (bulk
+//                                 copies) and scales page by page, up to four tiles ahead
 //
-// What is different from there, and why.  (1) The arithmetic per score bounds the kernel, so the V scale is folded into
-// the f16 V operand (one rounding of 2^-11, like a weight's) instead of riding in the exponent: no per-key additions
-// and multiplications in the softmax.  f16 holds vs * 448 only for vs in 2^-22 .. 2^-1 (with a common factor of 2^8);
-// a tile with a scale outside keeps the exponent form, and both forms add up in one accumulator.  (2) The running
-// maximum may lag the true one by up to 2^8: weights stay below 2^8, exact enough in f16, sums are fp32, and O is
-// rescaled a handful of times per row instead of on most tiles.  (3) Rows carry their own last visible key, pages may be
-// missing, and places that no row may see may hold anything: the tiles that reach past some row's last key (and only
-// those) replace NaN codes by zero and mark the key, so that exactly the rows that see it get NaN.
+// What is different from there, and why.
+// (1) K codes are operands as they lie in the cache: q is split into two E4M3 parts, q = hi + lo, and S = hi K^T + lo K^T.
+//     bf16 has 8 significant bits, E4M3 4: with the row scaled so that its largest |q| is in 128..256, every element
+//     above 2^-9 of it is exact, smaller ones are off by at most 2^-17 of it.  Two E4M3 products take the time of one f16
+//     product, and nothing has to convert K: clock stamps of the f16 form (0.80 ms on 8192 tokens, 32/8 heads of 128) had
+//     every product waiting for the converted K tile, and both row blocks in step behind it.
+// (2) The V scale is folded into the f16 V operand (one rounding of 2^-11, like a weight's) instead of riding in the
+//     exponent: no per-key additions and multiplications in the softmax.  f16 holds vs * 448 only for vs in 2^-22 .. 2^-1
+//     (with a common factor of 2^8); a tile with a scale outside keeps the exponent form, and both add up in one O.
+// (3) The running maximum may lag the true one by up to 2^8: weights stay below 2^8, exact enough in f16, sums are fp32,
+//     and O is rescaled a handful of times per row instead of on most tiles.
+// (4) Rows carry their own last visible key, pages may be missing, and places that no row may see may hold anything: the
+//     tiles that reach past some row's last key (and only those) replace NaN codes of V by zero and mark the key, so that
+//     exactly the rows that see it get NaN.
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "flash_prefill_roles.cuh"
 #include "flash_prefill_tc.cuh"
@@ -38,12 +47,41 @@ namespace paged {
 namespace {
 
 using namespace tc;
-using ws::group_or;
-using ws::kLazyNs;
-using ws::wait_phase;
 
-constexpr int kRawStages = 2;
-constexpr int kCstRing = 4;              // constants of a tile are read while those of the next two are written
+// Bounded wait on an mbarrier phase that also ends when another thread of the CTA has given up (ws::wait_phase's contract):
+// the common case, a phase that is complete or completes within a few polls, is a loop of two instructions.
+// kBackoffNs: pause after sixteen polls, for roles that are ahead (every poll goes through the shared-memory pipe).
+template <int kBackoffNs = 0>
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up, int where, int* error_word) {
+    const uint32_t addr = pipe::smem_u32(bar);
+    for (int i = 0; i < ws::kTries / 16; ++i) {
+        uint32_t left;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .u32 n;\n\tmov.u32 n, 16;\n"
+            "again%=:\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "@p bra done%=;\n\t"
+            "sub.u32 n, n, 1;\n\t"
+            "setp.ne.u32 p, n, 0;\n\t"
+            "@p bra again%=;\n"
+            "done%=:\n\t"
+            "mov.u32 %0, n;\n\t}"
+            : "=r"(left)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        // The lanes of a warp may see the phase complete on different polls: they meet again here, before instructions that
+        // want the whole warp.  (Called by whole warps.)
+        if (__all_sync(0xffffffffu, left != 0)) return true;
+        if (__any_sync(0xffffffffu, *gave_up != 0)) return false;
+        if constexpr (kBackoffNs > 0) __nanosleep(kBackoffNs);
+    }
+    *gave_up = 1;
+    if (error_word != nullptr) atomicCAS(error_word, 0, (where << 8) | 1);
+    return false;
+}
+
+constexpr int kStages = 4;               // tiles (K and V codes, scales) in flight or in use
+constexpr int kCstRing = 4;              // a tile's constants: read until its weights are out, at most two tiles after they were written
 constexpr int kFoldShift = 8;            // V operand = code * vs * 2^8
 constexpr float kFoldLow = 2.384185791015625e-07f;    // 2^-22
 constexpr float kFoldHigh = 0.5f;
@@ -77,41 +115,86 @@ struct Geo {
     static constexpr int kSoftmaxWarps = 8 * kBlocks;
     static constexpr int kIssuerWarp0 = kSoftmaxWarps;
     static constexpr int kConvWarp0 = kSoftmaxWarps + kBlocks;
-    static constexpr int kConvWarps = kBlocks == 1 ? 3 : 4;
-    static constexpr int kConvThreads = 32 * kConvWarps;
-    static constexpr int kCopyWarp = kConvWarp0 + kConvWarps;
+    static constexpr int kConvThreads = 128;
+    static constexpr int kCopyWarp = kConvWarp0 + kConvThreads / 32;
     static constexpr int kThreads = 32 * (kCopyWarp + 1);
     static constexpr int kPieces = kKeys * (D / 16);                        // 16-byte pieces of a raw tile
-    static constexpr int kPerConv = (kPieces + kConvThreads - 1) / kConvThreads;
+    static constexpr int kPerConv = kPieces / kConvThreads;
     static constexpr int kTmem = kTmemCols * kBlocks;
-    static constexpr int kDimBlocks = D / 64;
-    static constexpr int kQBytes = kDimBlocks * kRows * 128;
-    static constexpr int kTileBytes = kDimBlocks * kKeys * 128;             // an f16 operand tile
+    static constexpr int kDimBlocks = D / 64;                               // of the V operand
+    static constexpr int kQPart = kRows * D;                                // q hi (or lo) of a block: rows of D bytes
+    static constexpr int kTileBytes = kDimBlocks * kKeys * 128;             // an f16 V operand tile
     static constexpr int kRawBytes = kKeys * D;
-    static constexpr int kStageBytes = 2 * kRawBytes + 2 * kKeys * 4;       // raw K, raw V, K scales, V scales
+    static constexpr int kScaleAt = 2 * kRawBytes;                          // a stage: K codes, V codes, K scales, V scales (1 KB aligned)
+    static constexpr int kStageBytes = 2 * kRawBytes + 1024;
+    static constexpr int kCstFloats = 3 * kKeys + 4;                        // K scales; where V scales ride in the exponent: log2, inverse; flags
     static constexpr int kSQ = 0;
-    static constexpr int kSK = kSQ + kBlocks * kQBytes;
-    static constexpr int kSV = kSK + 2 * kTileBytes;
-    static constexpr int kSRaw = kSV + 2 * kTileBytes;
-    static constexpr int kCstFloats = 3 * kKeys + 4;                        // ksl, lgv, rvs, {flags}
-    static constexpr int kSCst = kSRaw + kRawStages * kStageBytes;
-    static constexpr int kSRow = kSCst + kCstRing * kCstFloats * 4;         // row maxima of |q| (two halves), later the rows' q factors
-    static constexpr int kSPoison = kSRow + kBlocks * 2 * kRows * 4;
-    static constexpr int kSBar = kSPoison + kKeys * 4;
-    static constexpr int kSmemBytes = kSBar + 256 + 1024;
-    static constexpr int kBarsPerBlock = 6;
-    static constexpr int kBarKReady = kBarsPerBlock * kBlocks;
-    static constexpr int kBarVReady = kBarKReady + 2;
-    static constexpr int kBarRawFull = kBarVReady + 2;
-    static constexpr int kBarRawEmpty = kBarRawFull + kRawStages;
-    static constexpr int kNumBars = kBarRawEmpty + kRawStages;
-    static_assert(8 * kNumBars + 32 <= 256, "barrier area");
+    static constexpr int kSK = kSQ + kBlocks * 2 * kQPart;
+    static constexpr int kSV = kSK + kStages * kStageBytes;
+    static constexpr int kSRow = kSV + 2 * kTileBytes;                      // per block: maxima of |q| (two halves of a row), then the rows' factors
+    static constexpr int kSCst = kSRow + kBlocks * 2 * kRows * 4;           // [kBlocks][kCstRing]
+    static constexpr int kSPoison = kSCst + kBlocks * kCstRing * kCstFloats * 4;   // per V buffer and key: 0, or NaN
+    static constexpr int kSBar = kSPoison + 2 * kKeys * 4;
+    static constexpr int kSmemBytes = kSBar + 512 + 1024;
+    static constexpr int kBarsPerBlock = 7;
+    static constexpr int kBarVReady = kBarsPerBlock * kBlocks;
+    static constexpr int kBarFull = kBarVReady + 2;
+    static constexpr int kBarEmpty = kBarFull + kStages;
+    static constexpr int kBarConv = kBarEmpty + kStages;
+    static constexpr int kNumBars = kBarConv + 1;
+    static_assert(8 * kNumBars + 4 * (4 + kStages) <= 512, "barrier area");
+    static_assert(kSK % 1024 == 0 && kStageBytes % 1024 == 0 && kSV % 1024 == 0 && kTileBytes % 1024 == 0, "operand tiles are 1 KB aligned");
 };
+// "W ready" exists once per W buffer: a warp may finish tile i + 1 (whose scores only wait for everyone to have READ those of
+// tile i) while another one still rescales O for tile i, and its arrival must not count for tile i.
 enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
 enum TileFlag { kSlow = 16 };            // flags: bits 0..3 = sixteen-key groups that exist, 16 = V scales ride in the exponent
 
-// the row of the K operand tile that holds key `key` of the tile (the inverse of ws::key_of_k_row)
-__device__ __forceinline__ int k_row_of_key(int key) { return (key & 48) | ((key & 2) << 2) | ((key & 12) >> 1) | (key & 1); }
+// Shared-memory descriptor of an E4M3 operand with rows of D bytes (K-major): 128-byte swizzle for D = 128, 64-byte for 64.
+template <int D>
+__device__ __forceinline__ uint64_t code_desc(uint32_t addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>((8 * D) >> 4) << 32;                         // eight rows
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(D == 128 ? 2 : 4) << 61;
+    return d;
+}
+// byte offset of 16-byte piece `piece` of row `row` in such an operand
+template <int D>
+__device__ __forceinline__ int code_at(int row, int piece) {
+    return D == 128 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// rows y .. of a [rows][D] byte array into shared memory, swizzled by the map; x is always 0
+__device__ __forceinline__ void tensor_load(void* dst, const CUtensorMap* map, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(pipe::smem_u32(dst)),
+                 "l"(map), "r"(0), "r"(y), "r"(pipe::smem_u32(bar))
+                 : "memory");
+}
+// true in one lane of the (whole) warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+// Whether a V scale is outside what the f16 operand holds.  (A NaN is not: it makes the operand NaN.)
+__device__ __forceinline__ bool outside_fold(float vs) { return vs != 0.0f && vs == vs && !(vs >= kFoldLow && vs <= kFoldHigh); }
+// two floats -> E4M3 codes hi and lo with x = hi + lo (lo: what hi leaves, rounded)
+__device__ __forceinline__ void split_e4m3x2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+    uint32_t back, none;
+    e4m3x4_to_f16x2x2(hi, back, none);
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&back));
+    lo = __nv_cvt_float2_to_fp8x2(make_float2(x - b.x, y - b.y), __NV_SATFINITE, __NV_E4M3);
+}
 
 // The batch entry and the token tile of CTA `index` (of all token tiles of all entries); false: there is none.
 // Tiles are numbered from the one with the most keys down, so the long ones start first: depth = keys in units of a
@@ -169,7 +252,7 @@ __device__ __forceinline__ bool find_tile(const BlockArgs& p, int index, int til
 
 // grid (kv heads x head chunks, token tiles, key ranges)
 template <int D, int kBlocks, bool kPrefix>
-__global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_kernel(const BlockArgs p) {
+__global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_kernel(const BlockArgs p, const __grid_constant__ CUtensorMap k_map) {
     using G = Geo<D, kBlocks>;
     extern __shared__ unsigned char raw_smem[];
     const uint32_t base = (pipe::smem_u32(raw_smem) + 1023u) & ~1023u;
@@ -177,10 +260,12 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + G::kSBar);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sm + G::kSBar + 8 * G::kNumBars);
     volatile int* const gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* const raw_groups = reinterpret_cast<int*>(tmem_slot + 2);       // [kRawStages] sixteen-key groups that were fetched
-    int* const least = raw_groups + kRawStages;                          // the CTA's least last visible key
+    int* const least = reinterpret_cast<int*>(tmem_slot + 2);            // prefix: the CTA's least last visible key
+    int* const stage_groups = reinterpret_cast<int*>(tmem_slot + 4);     // [kStages] sixteen-key groups that were fetched
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (through a shuffle, so that the compiler knows the warp's number and what follows from it to be uniform: the product
+    // warps' descriptors then live in uniform registers)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int kvh = blockIdx.x / p.head_chunks;
     const int chunk = blockIdx.x - kvh * p.head_chunks;
 
@@ -188,23 +273,22 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g) {
             uint64_t* const bb = bars + g * G::kBarsPerBlock;
-            pipe::mbar_init(&bb[kBarQK], 1);
-            pipe::mbar_init(&bb[kBarQK + 1], 1);
+            pipe::mbar_init(&bb[kBarQK], 2);              // the product's completion, and the product warp for the tile's constants
+            pipe::mbar_init(&bb[kBarQK + 1], 2);
             pipe::mbar_init(&bb[kBarPV], 1);
             pipe::mbar_init(&bb[kBarPV + 1], 1);
             pipe::mbar_init(&bb[kBarSRead], 8);
             pipe::mbar_init(&bb[kBarWReady], 8);
+            pipe::mbar_init(&bb[kBarWReady + 1], 8);
         }
+        pipe::mbar_init(&bars[G::kBarVReady], G::kConvThreads);
+        pipe::mbar_init(&bars[G::kBarVReady + 1], G::kConvThreads);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            pipe::mbar_init(&bars[G::kBarKReady + i], G::kConvThreads);
-            pipe::mbar_init(&bars[G::kBarVReady + i], G::kConvThreads);
+        for (int i = 0; i < kStages; ++i) {
+            pipe::mbar_init(&bars[G::kBarFull + i], 1 + 32);                    // the bulk copies' bytes, and the copy warp's lanes for their scales
+            pipe::mbar_init(&bars[G::kBarEmpty + i], kBlocks + G::kConvThreads / 32);
         }
-#pragma unroll
-        for (int i = 0; i < kRawStages; ++i) {
-            pipe::mbar_init(&bars[G::kBarRawFull + i], 1);
-            pipe::mbar_init(&bars[G::kBarRawEmpty + i], G::kConvThreads);
-        }
+        pipe::mbar_init(&bars[G::kBarConv], G::kConvThreads);
         *gave_up = 0;
         *least = INT_MAX;
         pipe::mbar_init_fence();
@@ -216,7 +300,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     // ---- what this CTA works on.  The prefix kernel follows a kernel of the same call whose results it does not need, and
     //      which has seen its own predecessors complete before this one may start: it waits at its end instead. ----
@@ -263,7 +347,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     const int block_tok = blk * p.tokens_per_block;          // first token of the block, counted from token0
     uint64_t* const bb = bars + blk * G::kBarsPerBlock;
     const uint32_t tmem_s = tmem + blk * kTmemCols, tmem_o = tmem_s + kKeys, tmem_w = tmem_o + kD;
-    const int q_off = G::kSQ + blk * G::kQBytes;
+    const int q_off = G::kSQ + blk * 2 * G::kQPart;
 
     // a row of a block: its head slot and token (counted from token0); whether it exists; the last key it sees
     auto row_at = [&](int row, int& tok, int& head) {
@@ -283,13 +367,18 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             return held + tok;
         }
     };
+    // the least last visible key of the CTA's rows: tiles beyond it hold keys that a row must not see
+    if constexpr (kPrefix) {
+        if (tid < min(tokens, tile_tokens)) atomicMin(least, last_key(tid));
+        __syncthreads();
+    }
+    const int seen_by_all = kPrefix ? *least : held;
 
-    // ---- Q (softmax warps): bf16 -> f16 into shared memory.  A row whose largest |q| f16 does not hold well is scaled by
-    //      a power of two, which its scores take back (rare; `scaled` is uniform over the block's warps). ----
-    bool scaled = false;
+    // ---- Q (softmax warps): bf16 -> two E4M3 parts in shared memory.  A row is scaled by a power of two so that its
+    //      largest |q| lies in 2^7 .. 2^8; its scores take that back. ----
     float* const row_amax = reinterpret_cast<float*>(sm + G::kSRow) + blk * 2 * kRows;
     if (warp < G::kSoftmaxWarps && n_tiles > 0) {
-        constexpr int kHalf = D / 16;                        // 16-byte pieces per thread: half a row
+        constexpr int kHalf = D / 16;                        // 16-byte pieces of bf16 per thread: half a row
         const int row = 32 * (wb & 3) + lane, part = wb >> 2;
         int tok, head;
         const bool valid = row_at(row, tok, head);
@@ -300,29 +389,37 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         for (int i = 0; i < kHalf; ++i) {
             w[i] = make_uint4(0u, 0u, 0u, 0u);
             if (valid) w[i] = src[i];
-            amax2 = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax2, w[i].x), w[i].y), w[i].z), w[i].w);
-        }
-        row_amax[part * kRows + row] = fmaxf(bf_lo(amax2), bf_hi(amax2));
-        named_sync(4 + blk, 256);
-        const float amax = fmaxf(row_amax[row], row_amax[kRows + row]);
-        const bool odd = amax > 0.0f && !(amax >= 0.015625f && amax < 32768.0f);     // outside 2^-6 .. 2^15
-        scaled = group_or(4 + blk, 256, odd);                // (also: everyone has read row_amax)
-        float down = 1.0f;
-        if (scaled) {
-            int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
-            e = odd ? max(-100, min(100, e)) : 0;
-            down = __int_as_float((127 - e) << 23);
-            if (part == 0) row_amax[row] = __int_as_float((127 + e) << 23);
         }
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) {
-            uint4 h;
-            h.x = pack_f16x2(bf_lo(w[i].x) * down, bf_hi(w[i].x) * down);
-            h.y = pack_f16x2(bf_lo(w[i].y) * down, bf_hi(w[i].y) * down);
-            h.z = pack_f16x2(bf_lo(w[i].z) * down, bf_hi(w[i].z) * down);
-            h.w = pack_f16x2(bf_lo(w[i].w) * down, bf_hi(w[i].w) * down);
-            const int piece = kHalf * part + i;
-            *reinterpret_cast<uint4*>(sm + q_off + (piece >> 3) * (kRows * 128) + swz128(row, piece & 7)) = h;
+        for (int i = 0; i < kHalf; ++i) amax2 = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax2, w[i].x), w[i].y), w[i].z), w[i].w);
+        const float lo_max = bf_lo(amax2), hi_max = bf_hi(amax2);
+        row_amax[part * kRows + row] = lo_max != lo_max ? lo_max : hi_max != hi_max ? hi_max : fmaxf(lo_max, hi_max);
+        named_sync(4 + blk, 256);
+        const float amax_a = row_amax[row], amax_b = row_amax[kRows + row];
+        const float amax = fmaxf(amax_a, amax_b);
+        named_sync(4 + blk, 256);                            // everyone has read the maxima
+        int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
+        e = amax > 0.0f ? max(-100, e) - 7 : 0;
+        float down = __int_as_float((127 - e) << 23);
+        // E4M3 conversion would saturate an infinite q: a row that holds one, or a NaN, gets NaN through its factor
+        const bool finite = amax_a <= 3.4e38f && amax_b <= 3.4e38f;
+        if (part == 0) row_amax[row] = finite ? fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23) : NAN;
+        if (p.scale_log2e < 0.0f) down = -down;
+#pragma unroll
+        for (int i = 0; i < kHalf / 2; ++i) {                // sixteen values: one 16-byte piece of each part
+            const uint32_t words[8] = {w[2 * i].x, w[2 * i].y, w[2 * i].z, w[2 * i].w, w[2 * i + 1].x, w[2 * i + 1].y, w[2 * i + 1].z, w[2 * i + 1].w};
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t h0, l0, h1, l1;
+                split_e4m3x2(bf_lo(words[2 * k]) * down, bf_hi(words[2 * k]) * down, h0, l0);
+                split_e4m3x2(bf_lo(words[2 * k + 1]) * down, bf_hi(words[2 * k + 1]) * down, h1, l1);
+                hi[k] = (h0 & 0xffffu) | (h1 << 16);
+                lo[k] = (l0 & 0xffffu) | (l1 << 16);
+            }
+            const int at = q_off + code_at<D>(row, (kHalf / 2) * part + i);
+            *reinterpret_cast<uint4*>(sm + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(sm + at + G::kQPart) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         fence_async_smem();
     }
@@ -338,67 +435,63 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         int tok_a, tok_b, head_a, head_b;
         const bool valid_a = row_at(row_a, tok_a, head_a), valid_b = row_at(row_b, tok_b, head_b);
         const int qpos_a = valid_a ? last_key(tok_a) : INT_MAX, qpos_b = valid_b ? last_key(tok_b) : INT_MAX;
-        const int qpos_min = min(qpos_a, qpos_b);
-        const float up_a = scaled ? row_amax[row_a] : 1.0f, up_b = scaled ? row_amax[row_b] : 1.0f;
+        const float c_a = n_tiles > 0 ? row_amax[row_a] : 0.0f, c_b = n_tiles > 0 ? row_amax[row_b] : 0.0f;
         float m_a = kMInit, m_b = kMInit, l_a = 0.0f, l_b = 0.0f;
-        bool ok = true;
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            ok = wait_phase(&bb[kBarQK + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word);
-            if (!ok) break;
-            tc_fence_after();
+        const float* const cst0 = reinterpret_cast<const float*>(sm + G::kSCst) + blk * kCstRing * G::kCstFloats;
+        // One tile.  The plain form (kAny false) is for tiles that every row sees whole and whose V
+        // scales are in the operand; kAny serves every tile.  Returns false when a wait gave up.
+        auto weigh = [&](auto any, int i, const float* cst, int flags) -> bool {
+            constexpr bool kAny = decltype(any)::value;
+            const int key0 = (j0 + i) * kKeys;
+            const bool slow = kAny && (flags & kSlow) != 0;
             uint32_t sr[32];
             tmem_ld_frag_x8(sr, tmem_s + my_lanes16);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bb[kBarSRead]);
-
-            const float* const cst = reinterpret_cast<const float*>(sm + G::kSCst) + (i & (kCstRing - 1)) * G::kCstFloats;
-            const int flags = reinterpret_cast<const int*>(cst)[3 * kKeys];
-            const int key0 = (j0 + i) * kKeys;
-            // pair 2 (2 a + h): row a, keys 16 a + 4 c2 + 2 h + {0, 1}; pair 2 (2 a + h) + 1: the same keys of row b
+            if (lane == 0) pipe::mbar_arrive(&bb[kBarSRead]);        // S may be overwritten by the next product
+            // pair 2 g: row a, keys 8 g + 2 c2 + {0, 1}; pair 2 g + 1: the same keys of row b.  (The constants lie in the
+            // order of the weights: four for g = 2 a, 2 a + 1 at 16 a + 4 c2.)
             float2 sv[16];
-            if (scaled) {
-#pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    sr[4 * g] = __float_as_uint(__uint_as_float(sr[4 * g]) * up_a);
-                    sr[4 * g + 1] = __float_as_uint(__uint_as_float(sr[4 * g + 1]) * up_a);
-                    sr[4 * g + 2] = __float_as_uint(__uint_as_float(sr[4 * g + 2]) * up_b);
-                    sr[4 * g + 3] = __float_as_uint(__uint_as_float(sr[4 * g + 3]) * up_b);
-                }
-            }
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const float4 kk = *reinterpret_cast<const float4*>(cst + 16 * a + 4 * c2);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int r = 4 * (2 * a + h);
+                    const int g = 2 * a + h;
                     const float2 k2 = h ? make_float2(kk.z, kk.w) : make_float2(kk.x, kk.y);
-                    sv[r / 2] = mul2_rn(make_float2(__uint_as_float(sr[r]), __uint_as_float(sr[r + 1])), k2);
-                    sv[r / 2 + 1] = mul2_rn(make_float2(__uint_as_float(sr[r + 2]), __uint_as_float(sr[r + 3])), k2);
+                    sv[2 * g] = mul2_rn(make_float2(__uint_as_float(sr[4 * g]), __uint_as_float(sr[4 * g + 1])), k2);
+                    sv[2 * g + 1] = mul2_rn(make_float2(__uint_as_float(sr[4 * g + 2]), __uint_as_float(sr[4 * g + 3])), k2);
                 }
             }
-            if (flags & kSlow) {                             // the V scales ride in the exponent on this tile
+            float f_a = c_a, f_b = c_b;
+            if constexpr (kAny) {
+                if (slow) {                                  // the V scales ride in the exponent on this tile
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const float4 lg = *reinterpret_cast<const float4*>(cst + kKeys + 16 * a + 4 * c2);
+                    for (int a = 0; a < 4; ++a) {
+                        const float4 lg = *reinterpret_cast<const float4*>(cst + kKeys + 16 * a + 4 * c2);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float x = h ? lg.z : lg.x, y = h ? lg.w : lg.y;
-                        const int g = 2 * a + h;
-                        sv[2 * g].x += x; sv[2 * g].y += y;
-                        sv[2 * g + 1].x += x; sv[2 * g + 1].y += y;
+                        for (int h = 0; h < 2; ++h) {
+                            const int g = 2 * a + h;
+                            const float x = h ? lg.z : lg.x, y = h ? lg.w : lg.y;
+                            sv[2 * g] = make_float2(fmaf(sv[2 * g].x, c_a, x), fmaf(sv[2 * g].y, c_a, y));
+                            sv[2 * g + 1] = make_float2(fmaf(sv[2 * g + 1].x, c_b, x), fmaf(sv[2 * g + 1].y, c_b, y));
+                        }
                     }
+                    f_a = f_b = 1.0f;
                 }
-            }
-            if (key0 + kKeys - 1 > qpos_min || (flags & 15) != 15) {
+                if (key0 + kKeys - 1 > seen_by_all || (flags & 15) != 15) {
+                    if (!wait_bar(&bars[G::kBarVReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word)) return false;   // marks of bad V rows
+                    const float* const poison = reinterpret_cast<const float*>(sm + G::kSPoison) + (i & 1) * kKeys + 2 * c2;
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    const int key = key0 + 16 * (g >> 1) + 4 * c2 + 2 * (g & 1);
-                    const bool gone = ((flags >> (g >> 1)) & 1) == 0;
-                    if (gone || key > qpos_a) sv[2 * g].x = -INFINITY;
-                    if (gone || key + 1 > qpos_a) sv[2 * g].y = -INFINITY;
-                    if (gone || key > qpos_b) sv[2 * g + 1].x = -INFINITY;
-                    if (gone || key + 1 > qpos_b) sv[2 * g + 1].y = -INFINITY;
+                    for (int g = 0; g < 8; ++g) {
+                        const int key = key0 + 8 * g + 2 * c2;
+                        const float2 bad = *reinterpret_cast<const float2*>(poison + 8 * g);
+                        const bool gone = ((flags >> (g >> 1)) & 1) == 0;
+                        sv[2 * g].x = gone || key > qpos_a ? -INFINITY : sv[2 * g].x + bad.x;
+                        sv[2 * g].y = gone || key + 1 > qpos_a ? -INFINITY : sv[2 * g].y + bad.y;
+                        sv[2 * g + 1].x = gone || key > qpos_b ? -INFINITY : sv[2 * g + 1].x + bad.x;
+                        sv[2 * g + 1].y = gone || key + 1 > qpos_b ? -INFINITY : sv[2 * g + 1].y + bad.y;
+                    }
                 }
             }
             float mx_a = fmaxf(sv[0].x, sv[0].y), mx_b = fmaxf(sv[1].x, sv[1].y);
@@ -407,13 +500,16 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 mx_a = fmaxf(mx_a, fmaxf(sv[2 * g].x, sv[2 * g].y));
                 mx_b = fmaxf(mx_b, fmaxf(sv[2 * g + 1].x, sv[2 * g + 1].y));
             }
-            mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
-            mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
-            mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
-            mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
+            mx_a *= f_a;
+            mx_b *= f_b;
+            // The maximum of the four threads of a row is only needed when one of them has left the old one too far behind.
             const bool moved = __any_sync(0xffffffffu, mx_a > m_a + kLag || mx_b > m_b + kLag);
             float corr_a = 1.0f, corr_b = 1.0f;
             if (moved) {                                     // every row of the warp follows its maximum
+                mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
+                mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
+                mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
+                mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
                 const float mn_a = fmaxf(m_a, mx_a), mn_b = fmaxf(m_b, mx_b);
                 corr_a = ex2f(m_a - mn_a);
                 corr_b = ex2f(m_b - mn_b);
@@ -422,39 +518,25 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 l_a *= corr_a;
                 l_b *= corr_b;
             }
-            const float2 neg_a = splat2(-m_a), neg_b = splat2(-m_b);
+            const float2 f2_a = splat2(f_a), f2_b = splat2(f_b), neg_a = splat2(-m_a), neg_b = splat2(-m_b);
             float2 sum_a = make_float2(0.0f, 0.0f), sum_b = make_float2(0.0f, 0.0f);
-            uint32_t wv[16];                 // word 4 a + h: row a, keys 16 a + 4 c2 + 2 h + {0, 1}; 4 a + 2 + h: row b
-            if (flags & kSlow) {
+            // word 4 (g / 2) + g % 2: row a, keys 8 g + 2 c2 + {0, 1}; + 2: row b.  In tensor memory that is pair 8 (g / 2) +
+            // 2 c2 + g % 2 of the row, so V's rows are laid out in that order.
+            uint32_t wv[16];
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const float4 rv = *reinterpret_cast<const float4*>(cst + 2 * kKeys + 16 * a + 4 * c2);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int g = 2 * a + h;
-                        const float2 r2 = h ? make_float2(rv.z, rv.w) : make_float2(rv.x, rv.y);
-                        const float2 xa = add2_rn(sv[2 * g], neg_a), xb = add2_rn(sv[2 * g + 1], neg_b);
-                        const float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y)), eb = make_float2(ex2f(xb.x), ex2f(xb.y));
-                        sum_a = fma2_rn(ea, r2, sum_a);
-                        sum_b = fma2_rn(eb, r2, sum_b);
-                        wv[4 * a + h] = pack_f16x2(ea.x, ea.y);
-                        wv[4 * a + 2 + h] = pack_f16x2(eb.x, eb.y);
-                    }
+            for (int g = 0; g < 8; ++g) {
+                const float2 xa = fma2_rn(sv[2 * g], f2_a, neg_a), xb = fma2_rn(sv[2 * g + 1], f2_b, neg_b);
+                const float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y)), eb = make_float2(ex2f(xb.x), ex2f(xb.y));
+                if (kAny && slow) {
+                    const float2 rv = *reinterpret_cast<const float2*>(cst + 2 * kKeys + 16 * (g >> 1) + 4 * c2 + 2 * (g & 1));
+                    sum_a = make_float2(sum_a.x + (ea.x == 0.0f ? 0.0f : ea.x * rv.x), sum_a.y + (ea.y == 0.0f ? 0.0f : ea.y * rv.y));
+                    sum_b = make_float2(sum_b.x + (eb.x == 0.0f ? 0.0f : eb.x * rv.x), sum_b.y + (eb.y == 0.0f ? 0.0f : eb.y * rv.y));
+                } else {
+                    sum_a = add2_rn(ea, sum_a);
+                    sum_b = add2_rn(eb, sum_b);
                 }
-            } else {
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int g = 2 * a + h;
-                        const float2 xa = add2_rn(sv[2 * g], neg_a), xb = add2_rn(sv[2 * g + 1], neg_b);
-                        const float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y)), eb = make_float2(ex2f(xb.x), ex2f(xb.y));
-                        sum_a = add2_rn(ea, sum_a);
-                        sum_b = add2_rn(eb, sum_b);
-                        wv[4 * a + h] = pack_f16x2(ea.x, ea.y);
-                        wv[4 * a + 2 + h] = pack_f16x2(eb.x, eb.y);
-                    }
-                }
+                wv[4 * (g >> 1) + (g & 1)] = pack_f16x2(ea.x, ea.y);
+                wv[4 * (g >> 1) + 2 + (g & 1)] = pack_f16x2(eb.x, eb.y);
             }
             l_a += sum_a.x + sum_a.y;
             l_b += sum_b.x + sum_b.y;
@@ -463,8 +545,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             // skipped on other tiles because no later product completes before this warp has signalled "W ready" for it.
             const bool rescale = moved && i > 0;
             if (rescale) {
-                ok = wait_phase(&bb[kBarPV + ((i - 1) & 1)], ((i - 1) >> 1) & 1, gave_up, __LINE__, p.error_word);
-                if (!ok) break;
+                if (!wait_bar(&bb[kBarPV + ((i - 1) & 1)], ((i - 1) >> 1) & 1, gave_up, __LINE__, p.error_word)) return false;
                 tc_fence_after();
             }
             tmem_st_frag_x4(tmem_w + (i & 1) * (kKeys / 2) + my_lanes16, wv);
@@ -486,14 +567,26 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                     tmem_st_frag_x8(tmem_o + my_lanes16 + cb, ov);
                 }
             }
+            return true;
+        };
+        bool ok = true;
+        for (int i = 0; i < n_tiles; ++i) {
+            ok = wait_bar(&bb[kBarQK + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word);
+            if (!ok) break;
+            tc_fence_after();
+            const float* const cst = cst0 + (i & (kCstRing - 1)) * G::kCstFloats;
+            const int flags = reinterpret_cast<const int*>(cst)[3 * kKeys];
+            if (flags == 15 && (j0 + i) * kKeys + kKeys - 1 <= seen_by_all) ok = weigh(std::false_type{}, i, cst, flags);
+            else ok = weigh(std::true_type{}, i, cst, flags);
+            if (!ok) break;
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bb[kBarWReady]);
+            if (lane == 0) pipe::mbar_arrive(&bb[kBarWReady + (i & 1)]);
         }
         // ---- epilogue: finished rows, or their states ----
         if (ok && n_tiles > 0)
-            ok = wait_phase(&bb[kBarPV + ((n_tiles - 1) & 1)], ((n_tiles - 1) >> 1) & 1, gave_up, __LINE__, p.error_word);
+            ok = wait_bar(&bb[kBarPV + ((n_tiles - 1) & 1)], ((n_tiles - 1) >> 1) & 1, gave_up, __LINE__, p.error_word);
         if (ok && work) {
             tc_fence_after();
             l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
@@ -537,215 +630,207 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         }
     } else if (warp < G::kConvWarp0) {
         // =============================== products of row block `blk` ===============================
-        constexpr uint32_t kIdescQK = instr_desc(kKeys, false);
+        constexpr uint32_t kIdescQK = instr_desc(kKeys, false);        // E4M3 operands have format number 0, as f16 has in its kind
         constexpr uint32_t kIdescPV = instr_desc(D, true);
+        const uint64_t q_hi = code_desc<D>(base + q_off), q_lo = code_desc<D>(base + q_off + G::kQPart);
+        const uint64_t k_tile = code_desc<D>(base + G::kSK), v_tile = smem_desc(base + G::kSV, kKeys * 128);
+        // S_t = hi K_t^T + lo K_t^T once K_t is there; the tile's constants go out with it, in the order of the weights
+        const int pos0 = ws::key_of_k_row(lane);             // the place of key `lane` (key 16 a + 8 h + 2 c + e lies at 16 a + 4 c + 2 h + e)
         auto issue_qk = [&](int t) {
+            const int stage = t % kStages;
+            if (!wait_bar(&bars[G::kBarFull + stage], (t / kStages) & 1, gave_up, __LINE__, p.error_word)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t k_base = base + G::kSK + (t & 1) * G::kTileBytes;
+            if (elect_one()) {
+                const uint64_t kd = k_tile + static_cast<uint64_t>(stage * (G::kStageBytes >> 4));
 #pragma unroll
-                for (int d = 0; d < G::kDimBlocks; ++d)
+                for (int s = 0; s < D / 32; ++s) umma_f8(tmem_s, q_hi + 2 * s, kd + 2 * s, kIdescQK, s > 0);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        umma_f16(tmem_s, smem_desc(base + q_off + d * (kRows * 128) + s * 32, 16), smem_desc(k_base + d * (kKeys * 128) + s * 32, 16),
-                                 kIdescQK, d > 0 || s > 0);
+                for (int s = 0; s < D / 32; ++s) umma_f8(tmem_s, q_lo + 2 * s, kd + 2 * s, kIdescQK, true);
                 umma_commit(&bb[kBarQK + (t & 1)]);
             }
+            const float* const ks = reinterpret_cast<const float*>(sm + G::kSK + stage * G::kStageBytes + G::kScaleAt);
+            float* const cst = reinterpret_cast<float*>(sm + G::kSCst) + (blk * kCstRing + (t & (kCstRing - 1))) * G::kCstFloats;
+            const int groups = stage_groups[stage], key0 = (j0 + t) * kKeys;
+            bool slow = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = lane + 32 * h;
+                cst[pos0 + 32 * h] = ks[key];
+                slow |= key0 + key < total_keys && ((groups >> (key >> 4)) & 1) && outside_fold(ks[kKeys + key]);
+            }
+            slow = __any_sync(0xffffffffu, slow);
+            if (slow) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float vs = ks[kKeys + lane + 32 * h];
+                    const float lg = fmaxf(lg2f(vs), kLgFloor) + static_cast<float>(kFoldShift);
+                    cst[kKeys + pos0 + 32 * h] = lg + vs * 0.0f;            // (the maximum loses a NaN scale: it is added back)
+                    cst[2 * kKeys + pos0 + 32 * h] = ex2f(-lg);
+                }
+            }
+            if (lane == 0) reinterpret_cast<int*>(cst)[3 * kKeys] = groups | (slow ? kSlow : 0);
             __syncwarp();
+            if (lane == 0) pipe::mbar_arrive(&bb[kBarQK + (t & 1)]);
+            return true;
         };
-        bool ok = n_tiles > 0 && wait_phase<kLazyNs>(&bars[G::kBarKReady], 0, gave_up, __LINE__, p.error_word);
-        if (ok) issue_qk(0);
+        bool ok = n_tiles > 0 && issue_qk(0);
         for (int i = 0; i < n_tiles && ok; ++i) {
             if (i + 1 < n_tiles) {
-                ok = wait_phase<kLazyNs>(&bb[kBarSRead], i & 1, gave_up, __LINE__, p.error_word) &&
-                     wait_phase<kLazyNs>(&bars[G::kBarKReady + ((i + 1) & 1)], ((i + 1) >> 1) & 1, gave_up, __LINE__, p.error_word);
+                ok = wait_bar(&bb[kBarSRead], i & 1, gave_up, __LINE__, p.error_word);
                 if (!ok) break;
-                issue_qk(i + 1);
+                if (lane == 0) pipe::mbar_arrive(&bars[G::kBarEmpty + i % kStages]);      // K_i's product is done, its scales are read
+                ok = issue_qk(i + 1);
+                if (!ok) break;
             }
-            ok = wait_phase<kLazyNs>(&bb[kBarWReady], i & 1, gave_up, __LINE__, p.error_word) &&
-                 wait_phase<kLazyNs>(&bars[G::kBarVReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word);
+            ok = wait_bar(&bb[kBarWReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word) &&
+                 wait_bar(&bars[G::kBarVReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t v_base = base + G::kSV + (i & 1) * G::kTileBytes;
+            if (elect_one()) {
+                const uint64_t vd = v_tile + static_cast<uint64_t>((i & 1) * (G::kTileBytes >> 4));
 #pragma unroll
                 for (int s = 0; s < kKeys / 16; ++s)
-                    umma_f16_ts(tmem_o, tmem_w + (i & 1) * (kKeys / 2) + s * 8, smem_desc(v_base + s * 2048, kKeys * 128), kIdescPV, i > 0 || s > 0);
+                    umma_f16_ts(tmem_o, tmem_w + (i & 1) * (kKeys / 2) + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
                 umma_commit(&bb[kBarPV + (i & 1)]);
             }
             __syncwarp();
         }
     } else if (warp < G::kCopyWarp) {
-        // =============================== conversion ===============================
+        // =============================== conversion of V ===============================
         constexpr int kPerRow = D / 16;
         const int t = tid - 32 * G::kConvWarp0;
-        // the least last visible key of the CTA's rows: tiles beyond it may hold keys that a row must not see
-        if constexpr (kPrefix) {
-            int mine = INT_MAX;
-            for (int tok = t; tok < min(tokens, tile_tokens); tok += G::kConvThreads) mine = min(mine, last_key(tok));
-            mine = __reduce_min_sync(0xffffffffu, mine);
-            if (lane == 0) atomicMin(least, mine);
-            named_sync(1, G::kConvThreads);
-        }
-        const int seen_by_all = kPrefix ? *least : held;
-        auto wait_blocks = [&](int which, int buf, uint32_t parity, int where) {
-            bool all = true;
-#pragma unroll
-            for (int g = 0; g < kBlocks; ++g)
-                all = all && wait_phase<kLazyNs>(&bars[g * G::kBarsPerBlock + which + buf], parity, gave_up, where, p.error_word);
-            return all;
+        float* const poison = reinterpret_cast<float*>(sm + G::kSPoison);
+        int met = 0;                                         // meetings of the conversion warps so far
+        auto meet = [&]() {                                  // bounded, unlike a named barrier: a thread that gave up does not come
+            pipe::mbar_arrive(&bars[G::kBarConv]);
+            return wait_bar(&bars[G::kBarConv], met++ & 1, gave_up, __LINE__, p.error_word);
         };
-        int* const poison = reinterpret_cast<int*>(sm + G::kSPoison);
         bool ok = true;
         for (int i = 0; i < n_tiles && ok; ++i) {
-            const int buf = i & 1, stage = i % kRawStages;
-            const uint32_t freed = ((i - 2) >> 1) & 1;
-            const unsigned char* const raw = sm + G::kSRaw + stage * G::kStageBytes;
-            const float* const raw_ks = reinterpret_cast<const float*>(raw + 2 * G::kRawBytes);
-            const float* const raw_vs = raw_ks + kKeys;
-            const int key0 = (j0 + i) * kKeys;
-            if (i >= 2) ok = wait_blocks(kBarQK, buf, freed, __LINE__);
-            ok = ok && wait_phase<kLazyNs>(&bars[G::kBarRawFull + stage], (i / kRawStages) & 1, gave_up, __LINE__, p.error_word);
-            if (group_or(1, G::kConvThreads, !ok)) { ok = false; break; }
-            const int groups = raw_groups[stage];
+            const int buf = i & 1, stage = i % kStages, key0 = (j0 + i) * kKeys;
+            const unsigned char* const raw = sm + G::kSK + stage * G::kStageBytes + G::kRawBytes;
+            const float* const raw_vs = reinterpret_cast<const float*>(sm + G::kSK + stage * G::kStageBytes + G::kScaleAt) + kKeys;
+            ok = wait_bar<50>(&bars[G::kBarFull + stage], (i / kStages) & 1, gave_up, __LINE__, p.error_word);
+            if (i >= 2) {        // the operand buffer is free once O += W_{i-2} V_{i-2} of every block is complete
+#pragma unroll
+                for (int g = 0; g < kBlocks; ++g)
+                    ok = ok && wait_bar<50>(&bars[g * G::kBarsPerBlock + kBarPV + buf], ((i - 2) >> 1) & 1, gave_up, __LINE__, p.error_word);
+            }
+            if (!ok) break;
+            const int groups = stage_groups[stage];
             const bool edge = key0 + kKeys - 1 > seen_by_all || groups != 15;      // uniform
-            if (edge) {          // keys whose V row holds a NaN code or has no finite scale: their scores become NaN, their row zero
-                if (t < kKeys) poison[t] = !(raw_vs[t] <= 3.0e38f);
-                named_sync(1, G::kConvThreads);
+            if (edge) {          // rows that hold a NaN code, or have no finite scale: zero, and marked for the scores
+                if (t < kKeys) poison[buf * kKeys + t] = raw_vs[t] <= 3.0e38f ? 0.0f : NAN;
+                if (!meet()) { ok = false; break; }
 #pragma unroll
                 for (int n = 0; n < G::kPerConv; ++n) {
                     const int c = t + G::kConvThreads * n;
-                    if (c < G::kPieces) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(raw + G::kRawBytes + c * 16);
-                        const uint32_t hit = (((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) |
-                                              ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
-                        if (hit != 0u) poison[c / kPerRow] = 1;
-                    }
+                    const uint4 w = *reinterpret_cast<const uint4*>(raw + c * 16);
+                    const uint32_t hit = (((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) |
+                                          ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
+                    if (hit != 0u) poison[buf * kKeys + c / kPerRow] = NAN;
                 }
-                named_sync(1, G::kConvThreads);
+                if (!meet()) { ok = false; break; }
             }
-            // whether some V scale is outside what the f16 operand holds (of the keys that count)
-            bool outside = false;
-            if (t < kKeys && key0 + t < total_keys && ((groups >> (t >> 4)) & 1) && !(edge && poison[t])) {
-                const float vs = raw_vs[t];
-                outside = vs != 0.0f && !(vs >= kFoldLow && vs <= kFoldHigh) && vs == vs;
-            }
-            const bool slow = group_or(1, G::kConvThreads, outside);
-            if (t < kKeys) {
-                float* const cst = reinterpret_cast<float*>(sm + G::kSCst) + (i & (kCstRing - 1)) * G::kCstFloats;
-                const bool none = (edge && poison[t]) || (slow && raw_vs[t] != raw_vs[t]);      // (the exponent form would lose a NaN scale)
-                cst[t] = none ? NAN : raw_ks[t] * p.scale_log2e;
-                if (slow) {
-                    const float lg = fmaxf(lg2f(raw_vs[t]), kLgFloor) + static_cast<float>(kFoldShift);
-                    cst[kKeys + t] = lg;
-                    cst[2 * kKeys + t] = ex2f(-lg);
-                }
-                if (t == 0) reinterpret_cast<int*>(cst)[3 * kKeys] = groups | (slow ? kSlow : 0);
-            }
+            auto counts = [&](int k) { return key0 + k < total_keys && ((groups >> (k >> 4)) & 1) && outside_fold(raw_vs[k]); };
+            const bool slow = __any_sync(0xffffffffu, counts(lane) || counts(lane + 32));      // as the product warps decide
             // E4M3 -> f16 operand rows: [dim block of 64][row][128 bytes, swizzled].  Consecutive threads take consecutive
             // pieces of the raw tile; the upper half of a row's pieces stores its second half first, so that the eight
             // threads of a row write eight different 16-byte columns.
-            unsigned char* const k_dst = sm + G::kSK + buf * G::kTileBytes;
             unsigned char* const v_dst = sm + G::kSV + buf * G::kTileBytes;
-            auto place = [&](unsigned char* tile, int row, int ch, const uint4& h0, const uint4& h1) {
-                unsigned char* const dst = tile + (ch >> 2) * (kKeys * 128) + swz128(row, 2 * (ch & 3));
-                const uintptr_t other = reinterpret_cast<uintptr_t>(dst) ^ 16;
+#pragma unroll
+            for (int n = 0; n < G::kPerConv; ++n) {
+                const int c = t + G::kConvThreads * n;
+                const int key = c / kPerRow, ch = c % kPerRow;
+                uint4 w = *reinterpret_cast<const uint4*>(raw + c * 16);
+                float vs = slow ? 1.0f : raw_vs[key] * static_cast<float>(1 << kFoldShift);
+                if (edge && (poison[buf * kKeys + key] != 0.0f || key0 + key >= total_keys || !((groups >> (key >> 4)) & 1))) {
+                    w = make_uint4(0u, 0u, 0u, 0u);
+                    vs = 0.0f;
+                }
+                const __half2 f = __float2half2_rn(vs);
+                uint32_t h[8];
+                e4m3x4_to_f16x2x2(w.x, h[0], h[1]);
+                e4m3x4_to_f16x2x2(w.y, h[2], h[3]);
+                e4m3x4_to_f16x2x2(w.z, h[4], h[5]);
+                e4m3x4_to_f16x2x2(w.w, h[6], h[7]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[e]), f);
+                    h[e] = *reinterpret_cast<const uint32_t*>(&x);
+                }
+                // key 16 a + 8 h + 2 c + e becomes row 16 a + 4 c + 2 h + e: the order in which the weights lie
+                const int row = ws::key_of_k_row(key);
+                unsigned char* const dst = v_dst + (ch >> 2) * (kKeys * 128) + swz128(row, 2 * (ch & 3));
+                const uintptr_t one = reinterpret_cast<uintptr_t>(dst), other = one ^ 16;
                 const bool second = (ch >> 2) & 1;
-                *reinterpret_cast<uint4*>(second ? other : reinterpret_cast<uintptr_t>(dst)) = second ? h1 : h0;
-                *reinterpret_cast<uint4*>(second ? reinterpret_cast<uintptr_t>(dst) : other) = second ? h0 : h1;
-            };
-#pragma unroll
-            for (int n = 0; n < G::kPerConv; ++n) {
-                const int c = t + G::kConvThreads * n;
-                if (c < G::kPieces) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(raw + c * 16);
-                    uint4 h0, h1;
-                    e4m3x4_to_f16x2x2(w.x, h0.x, h0.y);
-                    e4m3x4_to_f16x2x2(w.y, h0.z, h0.w);
-                    e4m3x4_to_f16x2x2(w.z, h1.x, h1.y);
-                    e4m3x4_to_f16x2x2(w.w, h1.z, h1.w);
-                    place(k_dst, k_row_of_key(c / kPerRow), c % kPerRow, h0, h1);
-                }
-            }
-            fence_async_smem();
-            pipe::mbar_arrive(&bars[G::kBarKReady + buf]);
-            // V of the tile, once O += W_{i-2} V_{i-2} is complete
-            if (i >= 2) ok = wait_blocks(kBarPV, buf, freed, __LINE__);
-            if (group_or(1, G::kConvThreads, !ok)) { ok = false; break; }
-#pragma unroll
-            for (int n = 0; n < G::kPerConv; ++n) {
-                const int c = t + G::kConvThreads * n;
-                if (c < G::kPieces) {
-                    const int key = c / kPerRow;
-                    uint4 w = *reinterpret_cast<const uint4*>(raw + G::kRawBytes + c * 16);
-                    float vs = slow ? 1.0f : raw_vs[key] * static_cast<float>(1 << kFoldShift);
-                    if (edge && (poison[key] || key0 + key >= total_keys || !((groups >> (key >> 4)) & 1))) {
-                        w = make_uint4(0u, 0u, 0u, 0u);
-                        vs = 0.0f;
-                    }
-                    const __half2 f = __float2half2_rn(vs);
-                    uint32_t h[8];
-                    e4m3x4_to_f16x2x2(w.x, h[0], h[1]);
-                    e4m3x4_to_f16x2x2(w.y, h[2], h[3]);
-                    e4m3x4_to_f16x2x2(w.z, h[4], h[5]);
-                    e4m3x4_to_f16x2x2(w.w, h[6], h[7]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[e]), f);
-                        h[e] = *reinterpret_cast<const uint32_t*>(&x);
-                    }
-                    place(v_dst, key, c % kPerRow, make_uint4(h[0], h[1], h[2], h[3]), make_uint4(h[4], h[5], h[6], h[7]));
-                }
+                const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+                *reinterpret_cast<uint4*>(second ? other : one) = second ? h1 : h0;
+                *reinterpret_cast<uint4*>(second ? one : other) = second ? h0 : h1;
             }
             fence_async_smem();
             pipe::mbar_arrive(&bars[G::kBarVReady + buf]);
-            pipe::mbar_arrive(&bars[G::kBarRawEmpty + stage]);
+            __syncwarp();
+            if (lane == 0) pipe::mbar_arrive(&bars[G::kBarEmpty + stage]);
         }
     } else {
         // =============================== copies ===============================
-        // A tile is one run per page and array: lane (array, run) of K codes, V codes, K scales, V scales.
+        // A tile is one run of keys per page: lane r looks up run r's page, one elected lane issues a run's two copies.  The
+        // scales (256 bytes each of K and V) come by ordinary asynchronous copies, 16 bytes per lane.
         const int shift = p.c.page_shift;
-        const int run_keys = shift < 6 ? 1 << shift : kKeys, runs = kKeys / run_keys;
-        const int array = lane / runs, run = lane - array * runs;
+        const int run_shift = shift < 6 ? shift : 6, run_keys = 1 << run_shift, runs = kKeys >> run_shift;
+        const int my_key = lane < runs ? lane << run_shift : 0;      // first key of this lane's run
+        const int scale_key = 4 * (lane & 15);                       // the four keys whose scales this lane copies
+        const float* const scales = lane < 16 ? p.c.k_scale : p.c.v_scale;
         auto page_of = [&](int i) {
-            const int key = (j0 + i) * kKeys + run * run_keys;
+            const int key = (j0 + i) * kKeys + my_key;
             int id = -1;
-            if (lane < 4 * runs && i < n_tiles && key < total_keys && (key >> shift) < p.c.pages_per_row) id = pages[key >> shift];
+            if (lane < runs && i < n_tiles && key < total_keys && (key >> shift) < p.c.pages_per_row) id = pages[key >> shift];
             return id >= 0 && id < p.c.num_pages ? id : -1;
         };
-        const int per_key = array < 2 ? D : 4;
-        const uint32_t bytes = static_cast<uint32_t>(run_keys * per_key);
-        const unsigned char* const src0 = array == 0 ? p.c.k : array == 1 ? p.c.v : array == 2 ? reinterpret_cast<const unsigned char*>(p.c.k_scale)
-                                                                                               : reinterpret_cast<const unsigned char*>(p.c.v_scale);
-        const int dst0 = (array < 2 ? array * G::kRawBytes : 2 * G::kRawBytes + (array - 2) * kKeys * 4) + run * static_cast<int>(bytes);
-        int next = page_of(0);
+        int id = page_of(0), next = page_of(1);
         int issued = 0;
         bool ok = true;
         for (int i = 0; i < n_tiles; ++i) {
-            const int id = next;
-            next = page_of(i + 1);
-            const int stage = i % kRawStages;
-            if (i >= kRawStages) ok = wait_phase<kLazyNs>(&bars[G::kBarRawEmpty + stage], ((i / kRawStages) - 1) & 1, gave_up, __LINE__, p.error_word);
+            const int stage = i % kStages, after = page_of(i + 2);
+            const unsigned have = __ballot_sync(0xffffffffu, id >= 0);               // the runs of the tile that exist
+            if (i >= kStages) ok = wait_bar<50>(&bars[G::kBarEmpty + stage], ((i / kStages) - 1) & 1, gave_up, __LINE__, p.error_word);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            const unsigned have = __ballot_sync(0xffffffffu, id >= 0);      // bits 0 .. runs-1: the runs of the tile that exist
-            int groups = 0;
-            for (int r = 0; r < runs; ++r)
-                if ((have >> r) & 1) groups |= ((1 << (run_keys / 16)) - 1) << (r * (run_keys / 16));
-            if (lane == 0) {
-                raw_groups[stage] = groups;
-                pipe::mbar_expect_tx(&bars[G::kBarRawFull + stage], static_cast<uint32_t>(__popc(have & ((1u << runs) - 1u)) * run_keys * (2 * D + 8)));
+            unsigned char* const dst = sm + G::kSK + stage * G::kStageBytes;
+            uint64_t* const full = &bars[G::kBarFull + stage];
+            if (elect_one()) {
+                int groups = 0;
+                for (int r = 0; r < runs; ++r)
+                    if ((have >> r) & 1) groups |= ((1 << (run_keys >> 4)) - 1) << (r * (run_keys >> 4));
+                stage_groups[stage] = groups;
+                pipe::mbar_expect_tx(full, static_cast<uint32_t>((__popc(have) << run_shift) * 2 * D));
             }
             __syncwarp();
-            if (id >= 0) {
-                const size_t key = key_index(p.c, id, kvh) + (((j0 + i) * kKeys + run * run_keys) & ((1 << shift) - 1));
-                pipe::bulk_load(sm + G::kSRaw + stage * G::kStageBytes + dst0, src0 + key * per_key, bytes, &bars[G::kBarRawFull + stage]);
+            const int in_page = ((j0 + i) * kKeys) & ((1 << shift) - 1);             // (0 for pages of at most a tile)
+            for (int r = 0; r < runs; ++r) {
+                const int page = __shfl_sync(0xffffffffu, id, r);
+                if (page >= 0 && elect_one()) {
+                    const size_t key = key_index(p.c, page, kvh) + in_page;
+                    const int at = (r << run_shift) * D;
+                    tensor_load(dst + at, &k_map, static_cast<int>(key), full);
+                    pipe::bulk_load(dst + G::kRawBytes + at, p.c.v + key * D, static_cast<uint32_t>(D << run_shift), full);
+                }
+                __syncwarp();
+            }
+            {
+                const int page = __shfl_sync(0xffffffffu, id, scale_key >> run_shift);
+                const size_t key = page >= 0 ? key_index(p.c, page, kvh) + in_page + (scale_key & (run_keys - 1)) : 0;
+                cp16_zfill(pipe::smem_u32(dst + G::kScaleAt + (lane >> 4) * (kKeys * 4) + scale_key * 4), scales + key, page >= 0);
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pipe::smem_u32(full)) : "memory");
             }
             issued = i + 1;
+            id = next;
+            next = after;
         }
         if (!ok)        // somebody gave up: let the copies on their way land (bounded again) before the CTA ends
-            for (int i = max(0, issued - kRawStages); i < issued; ++i) {
-                for (int tries = 0; tries < (1 << 12) && !pipe::mbar_try_wait(&bars[G::kBarRawFull + i % kRawStages], (i / kRawStages) & 1); ++tries) {}
-            }
+            for (int i = max(0, issued - kStages); i < issued; ++i)
+                for (int tries = 0; tries < (1 << 12) && !pipe::mbar_try_wait(&bars[G::kBarFull + i % kStages], (i / kStages) & 1); ++tries) {}
+        cp_async_wait<0>();
     }
 
     // ---- common exit ----
@@ -800,12 +885,40 @@ void deal_heads(int group, BlockArgs& a) {
     a.tokens_per_block = kRows / a.heads_per_cta;
 }
 
+// The K codes of a layer as rows of head_dim bytes, copied in boxes of one run of keys, swizzled as the products read them.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int make_k_map(const Layer& c, int head_dim, const char* fn, CUtensorMap* map) {
+    static const EncodeTiled encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    RH_REQUIRE(encode != nullptr, RH_ERR_CUDA, "%s: the driver has no cuTensorMapEncodeTiled", fn);
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), (static_cast<cuuint64_t>(c.num_pages) * c.num_kv_heads) << c.page_shift};
+    RH_REQUIRE(dims[1] <= INT_MAX, RH_ERR_UNSUPPORTED_DIM, "%s: a layer must hold fewer than 2^31 keys x kv heads", fn);
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim)};
+    const int page = 1 << c.page_shift;
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(head_dim), static_cast<cuuint32_t>(page < kKeys ? page : kKeys)}, steps[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.k, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    RH_REQUIRE(r == CUDA_SUCCESS, RH_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", fn, static_cast<int>(r));
+    return RH_OK;
+}
+
 template <int D, int kBlocks, bool kPrefix>
 int launch_blocks_as(const BlockArgs& a, unsigned tiles, unsigned splits, cudaStream_t stream, const char* fn) {
     using G = Geo<D, kBlocks>;
     const dim3 grid(static_cast<unsigned>(a.c.num_kv_heads * a.head_chunks), tiles, splits);
+    CUtensorMap map;
+    if (const int e = make_k_map(a.c, D, fn, &map)) return e;
     (void)host::setup<&paged_blocks_kernel<D, kBlocks, kPrefix>, G::kThreads, G::kSmemBytes>();
-    host::launch<paged_blocks_kernel<D, kBlocks, kPrefix>>(grid, dim3(G::kThreads), static_cast<size_t>(G::kSmemBytes), stream, a);
+    host::launch<paged_blocks_kernel<D, kBlocks, kPrefix>>(grid, dim3(G::kThreads), static_cast<size_t>(G::kSmemBytes), stream, a, map);
     return host::check_launch(fn);
 }
 
@@ -862,7 +975,7 @@ int launch_prefix(const DecodeArgs& d, int head_dim, cudaStream_t stream, const 
     a.out_rows = static_cast<long long>(d.num_seqs) * a.num_q_heads;
     a.num_tokens = d.num_seqs;
     a.num_seqs = d.num_seqs;
-    a.scale_log2e = d.scale_log2e;
+    a.scale_log2e = d.scale_log2e == 0.0f ? 1.0e-30f : d.scale_log2e;
     deal_heads(d.group, a);
     const int blocks = d.num_seqs > a.tokens_per_block ? 2 : 1;
     const unsigned tiles = static_cast<unsigned>((d.num_seqs + blocks * a.tokens_per_block - 1) / (blocks * a.tokens_per_block));
@@ -932,7 +1045,7 @@ extern "C" int rh_flash_prefill_packed_bf16(void* out, const void* q, long long 
     a.out_rows = static_cast<long long>(num_tokens) * num_q_heads;
     a.num_tokens = num_tokens;
     a.num_seqs = num_seqs;
-    a.scale_log2e = scale * paged::kLog2e;
+    a.scale_log2e = scale == 0.0f ? 1.0e-30f : scale * paged::kLog2e;      // (a masked score times zero would be NaN)
     paged::deal_heads(num_q_heads / cache->num_kv_heads, a);
     if (num_splits > 1) {
         a.state_acc = partial_or_null;

@@ -158,7 +158,7 @@ def attend(q, k, v, first, scale):
     return o.permute(1, 0, 2)
 
 
-def check_attention(out, q, k, v, first, scale, what="", extra=0.0, small_step=2.0 ** -34, mixed=False):
+def check_attention(out, q, k, v, first, scale, what="", extra=0.0, small_step=2.0 ** -34, mixed=False, q_step=0.0):
     """Holds tokens `out` [n, heads, D] (bf16) against attend() in 64 bits, within what the arithmetic allows, derived:
 
       the store            a bf16 rounding                                                    2^-8 |o|
@@ -169,6 +169,7 @@ def check_attention(out, q, k, v, first, scale, what="", extra=0.0, small_step=2
       small weights        f16 loses what is below 2^-24 in units where the largest is 2^10   n 2^-34 max |v|   (`small_step`: 2^-25
                            where the largest weight may be 1: half a step of 2^-24)
       `extra`              of A, for forms that round once more
+      `q_step`             of max |q| sum_d |k_jd|, for a form that rounds q: joins the scores' error
       `mixed`              keys whose V scale rides in the exponent beside keys whose scale is folded into V, times 2^8: the
                            latter's weights are taken relative to a maximum that is up to 2^(lg vs + 8) higher, |v| <= 224:
                            n 2^-25 2^7 max_i p_i max |v_i|
@@ -186,7 +187,9 @@ def check_attention(out, q, k, v, first, scale, what="", extra=0.0, small_step=2
     p = torch.exp(zz - torch.where(torch.isinf(m), torch.zeros_like(m), m))
     p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
     a = torch.einsum("hnk,hkd->hnd", p, fv.abs())
-    delta = 2.0 * (2.0 ** -18 * big + 2.0 ** -21 * (top + 40.0))
+    sums = torch.where(seen, fk.abs().sum(-1)[:, None], torch.zeros_like(z)).amax(-1, keepdim=True)
+    rounded = q_step * abs(scale) * q.double().abs().amax(-1).t().unsqueeze(-1) * sums
+    delta = 2.0 * (2.0 ** -18 * big + rounded + 2.0 ** -21 * (top + 40.0))
     small = kk.shape[1] * small_step * fv.abs().amax((-2, -1), keepdim=True)
     if mixed:
         small = small + kk.shape[1] * 2.0 ** -18 * (p * fv.abs().amax(-1)[:, None]).amax(-1, keepdim=True)

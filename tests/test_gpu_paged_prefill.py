@@ -1,5 +1,6 @@
 """rh_flash_prefill_packed_bf16 against attention in 64 bits over what the pages hold (paged_util.check_attention derives the
-tolerance; the V operand is rounded to f16 once more here, 2^-11 of each term, and the scale it is multiplied with as well)."""
+tolerance; here the V operand is rounded to f16 once more, 2^-11 of each term, as is the scale it is multiplied with, and q is
+the sum of two E4M3 parts, off by at most 2^-17 of the row's largest value)."""
 import math
 
 import pytest
@@ -10,7 +11,7 @@ from test_gpu_paged_decode import filled, queries
 
 pytestmark = pytest.mark.gpu
 
-HOLD = dict(extra=2.0 * 2.0 ** -11, small_step=2.0 ** -25)      # the V operand: f16 of (code x f16 of the scale)
+HOLD = dict(extra=2.0 * 2.0 ** -11, small_step=2.0 ** -25, q_step=2.0 ** -17)      # the V operand: f16 of (code x f16 of the scale)
 
 
 def prefill(c, q, cu, num_q, scale, splits=1, rows=None, layer=0, out=None, total=None, num_seqs=None):
@@ -135,6 +136,27 @@ def test_extreme_scales_and_queries():
     check(c, prefill(c, q, cu, hq, scale), q, [n], [0], scale, mixed=True)
     q *= 1e28
     check(c, prefill(c, q, cu, hq, scale * 1e-28), q, [n], [0], scale * 1e-28, mixed=True)
+    q[7, 2, 5], q[9, 1, 0] = float("inf"), float("nan")
+    out = prefill(c, q, cu, hq, scale * 1e-28)
+    assert torch.isnan(out[7, 2]).all() and torch.isnan(out[9, 1]).all()
+    q[7, 2, 5], q[9, 1, 0] = 0, 0
+    out[7, 2], out[9, 1] = prefill(c, q, cu, hq, scale * 1e-28)[7, 2], prefill(c, q, cu, hq, scale * 1e-28)[9, 1]
+    check(c, out, q, [n], [0], scale * 1e-28, mixed=True)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_softmax_scale_of_zero_and_below(scale):
+    c, q, cu = batch([70, 5], [0, 40], 8, 2, 128, 16, seed=11)
+    check(c, prefill(c, q, cu, 8, scale), q, [70, 5], [0, 40], scale)
+
+
+def test_queries_of_widely_different_size_in_a_row():
+    """Elements far below a row's largest one: what the two parts of q lose must stay within 2^-17 of it."""
+    hq, hkv, dim = 8, 2, 128
+    c, q, cu = batch([150], [30], hq, hkv, dim, 32, seed=13)
+    q *= torch.exp2(-torch.randint(0, 22, q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).float()).to(torch.bfloat16)
+    for mul in (1.0, 200.0):
+        check(c, prefill(c, q * mul, cu, hq, 0.1), q * mul, [150], [30], 0.1)
 
 
 def test_long_prompt_sampled_tokens_and_repeatability():
