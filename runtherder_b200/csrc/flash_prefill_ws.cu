@@ -66,13 +66,15 @@ struct Geo {
     static constexpr int kSCst = kSRawS + 2 * kKeys * 4;             // ring of {ksl[64], lgv[64], rvs[64]}
     static constexpr int kSBar = kSCst + kCstRing * 3 * kKeys * 4;   // mbarriers, tensor-memory base, give-up flag
     static constexpr int kSmemBytes = kSBar + 256 + 1024;
-    // mbarriers: per row block {S complete x2, O += W V complete x2, S read, W ready}, then K ready x2, V ready x2;
+    // mbarriers: per row block {S complete x2, O += W V complete x2, S read, W ready x2}, then K ready x2, V ready x2;
     // tile j uses entry j % 2 of the paired ones, in that entry's phase j / 2
-    static constexpr int kBarsPerBlock = 6;
+    static constexpr int kBarsPerBlock = 7;
     static constexpr int kBarKReady = kBarsPerBlock * kBlocks;
     static constexpr int kBarVReady = kBarKReady + 2;
     static constexpr int kNumBars = kBarVReady + 2;
 };
+// "W ready" exists once per W buffer: a warp may finish tile j + 1 (whose scores only wait for everyone to have READ those of
+// tile j) while another one still rescales O for tile j, and its arrival must not count for tile j.
 enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
 
 // Probe of the give-up path of wait_phase (rh_selfcheck_role_wait): warp 0 waits with a limit of `tries` on a
@@ -129,6 +131,7 @@ __global__ void __launch_bounds__(Geo<kBlocks>::kThreads, 1) flash_prefill_ws_ke
             pipe::mbar_init(&bb[kBarPV + 1], 1);
             pipe::mbar_init(&bb[kBarSRead], 8);
             pipe::mbar_init(&bb[kBarWReady], 8);
+            pipe::mbar_init(&bb[kBarWReady + 1], 8);
         }
         pipe::mbar_init(&bars[G::kBarKReady], G::kConvThreads);
         pipe::mbar_init(&bars[G::kBarKReady + 1], G::kConvThreads);
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(Geo<kBlocks>::kThreads, 1) flash_prefill_ws_ke
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bb[kBarWReady]);
+            if (lane == 0) pipe::mbar_arrive(&bb[kBarWReady + (j & 1)]);
         }
         // ---- epilogue: normalise and store this thread's two rows ----
         if (ok && n_tiles > 0)
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(Geo<kBlocks>::kThreads, 1) flash_prefill_ws_ke
                 if (!ok) break;
                 issue_qk(j + 1);
             }
-            ok = wait_phase<kLazyNs>(&bb[kBarWReady], j & 1, gave_up, __LINE__, p.error_word) &&
+            ok = wait_phase<kLazyNs>(&bb[kBarWReady + (j & 1)], (j >> 1) & 1, gave_up, __LINE__, p.error_word) &&
                  wait_phase<kLazyNs>(&bars[G::kBarVReady + (j & 1)], (j >> 1) & 1, gave_up, __LINE__, p.error_word);
             if (!ok) break;
             tc_fence_after();
