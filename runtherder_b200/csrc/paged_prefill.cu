@@ -12,8 +12,8 @@
 //   O[128 x D] += W V        f16 (kind::f16): W = 2^(S c ks - m) in tensor memory, V = code x V scale in shared memory
 //
 //   softmax warps (8 per block)   scores -> weights; two rows x sixteen keys per thread
-//   product warp (1 per block)    issues the products
-//   conversion warps (4)          raw E4M3 V tiles -> f16 operand tiles, scales folded in
+//   product warps                 one thread issues S = Q K^T (of both blocks in turn), one per block O += W V
+//   conversion warps (4)          raw E4M3 V tiles -> f16 operand tiles, scales folded in; a tile's constants for the softmax
 //   copy warp                     fetches K tiles (tensor-map copies, swizzled as the product wants them), V tiles (bulk
 //                                 copies) and scales page by page, up to four tiles ahead
 //
@@ -50,7 +50,7 @@ using namespace tc;
 
 // Bounded wait on an mbarrier phase that also ends when another thread of the CTA has given up (ws::wait_phase's contract):
 // the common case, a phase that is complete or completes within a few polls, is a loop of two instructions.
-// kBackoffNs: pause after sixteen polls, for roles that are ahead (every poll goes through the shared-memory pipe).
+// (Called by whole warps.)  kBackoffNs: pause after sixteen polls, for roles that are ahead (every poll goes through the shared-memory pipe).
 template <int kBackoffNs = 0>
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up, int where, int* error_word) {
     const uint32_t addr = pipe::smem_u32(bar);
@@ -70,7 +70,7 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
             : "r"(addr), "r"(parity)
             : "memory");
         // The lanes of a warp may see the phase complete on different polls: they meet again here, before instructions that
-        // want the whole warp.  (Called by whole warps.)
+        // want the whole warp.
         if (__all_sync(0xffffffffu, left != 0)) return true;
         if (__any_sync(0xffffffffu, *gave_up != 0)) return false;
         if constexpr (kBackoffNs > 0) __nanosleep(kBackoffNs);
@@ -80,6 +80,7 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
     return false;
 }
 
+constexpr int kVBuffers = 3;             // f16 V operand tiles
 constexpr int kStages = 4;               // tiles (K and V codes, scales) in flight or in use
 constexpr int kCstRing = 4;              // a tile's constants: read until its weights are out, at most two tiles after they were written
 constexpr int kFoldShift = 8;            // V operand = code * vs * 2^8
@@ -114,7 +115,7 @@ template <int D, int kBlocks>
 struct Geo {
     static constexpr int kSoftmaxWarps = 8 * kBlocks;
     static constexpr int kIssuerWarp0 = kSoftmaxWarps;
-    static constexpr int kConvWarp0 = kSoftmaxWarps + kBlocks;
+    static constexpr int kConvWarp0 = kSoftmaxWarps + 1 + kBlocks;          // one warp for S, one per block for O (24 warps: 80 registers each)
     static constexpr int kConvThreads = 128;
     static constexpr int kCopyWarp = kConvWarp0 + kConvThreads / 32;
     static constexpr int kThreads = 32 * (kCopyWarp + 1);
@@ -131,16 +132,18 @@ struct Geo {
     static constexpr int kSQ = 0;
     static constexpr int kSK = kSQ + kBlocks * 2 * kQPart;
     static constexpr int kSV = kSK + kStages * kStageBytes;
-    static constexpr int kSRow = kSV + 2 * kTileBytes;                      // per block: maxima of |q| (two halves of a row), then the rows' factors
-    static constexpr int kSCst = kSRow + kBlocks * 2 * kRows * 4;           // [kBlocks][kCstRing]
-    static constexpr int kSPoison = kSCst + kBlocks * kCstRing * kCstFloats * 4;   // per V buffer and key: 0, or NaN
-    static constexpr int kSBar = kSPoison + 2 * kKeys * 4;
+    static constexpr int kSRow = kSV + kVBuffers * kTileBytes;                    // per block: maxima of |q| (two halves of a row), then the rows' factors
+    static constexpr int kSCst = kSRow + kBlocks * 2 * kRows * 4;           // [kCstRing]
+    static constexpr int kSPoison = kSCst + kCstRing * kCstFloats * 4;      // per V buffer and key: 0, or NaN
+    static constexpr int kSBar = kSPoison + kVBuffers * kKeys * 4;
     static constexpr int kSmemBytes = kSBar + 512 + 1024;
     static constexpr int kBarsPerBlock = 7;
     static constexpr int kBarVReady = kBarsPerBlock * kBlocks;
-    static constexpr int kBarFull = kBarVReady + 2;
+    static constexpr int kBarVEmpty = kBarVReady + kVBuffers;
+    static constexpr int kBarFull = kBarVEmpty + kVBuffers;
     static constexpr int kBarEmpty = kBarFull + kStages;
-    static constexpr int kBarConv = kBarEmpty + kStages;
+    static constexpr int kBarCst = kBarEmpty + kStages;
+    static constexpr int kBarConv = kBarCst + kCstRing;
     static constexpr int kNumBars = kBarConv + 1;
     static_assert(8 * kNumBars + 4 * (4 + kStages) <= 512, "barrier area");
     static_assert(kSK % 1024 == 0 && kStageBytes % 1024 == 0 && kSV % 1024 == 0 && kTileBytes % 1024 == 0, "operand tiles are 1 KB aligned");
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
 #pragma unroll
         for (int g = 0; g < kBlocks; ++g) {
             uint64_t* const bb = bars + g * G::kBarsPerBlock;
-            pipe::mbar_init(&bb[kBarQK], 2);              // the product's completion, and the product warp for the tile's constants
+            pipe::mbar_init(&bb[kBarQK], 2);              // the product's completion, and the product thread for the rest that the tile needs
             pipe::mbar_init(&bb[kBarQK + 1], 2);
             pipe::mbar_init(&bb[kBarPV], 1);
             pipe::mbar_init(&bb[kBarPV + 1], 1);
@@ -281,13 +284,18 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             pipe::mbar_init(&bb[kBarWReady], 8);
             pipe::mbar_init(&bb[kBarWReady + 1], 8);
         }
-        pipe::mbar_init(&bars[G::kBarVReady], G::kConvThreads);
-        pipe::mbar_init(&bars[G::kBarVReady + 1], G::kConvThreads);
+#pragma unroll
+        for (int i = 0; i < kVBuffers; ++i) {
+            pipe::mbar_init(&bars[G::kBarVReady + i], G::kConvThreads);
+            pipe::mbar_init(&bars[G::kBarVEmpty + i], kBlocks);
+        }
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
             pipe::mbar_init(&bars[G::kBarFull + i], 1 + 32);                    // the bulk copies' bytes, and the copy warp's lanes for their scales
-            pipe::mbar_init(&bars[G::kBarEmpty + i], kBlocks + G::kConvThreads / 32);
+            pipe::mbar_init(&bars[G::kBarEmpty + i], 1 + G::kConvThreads / 32);           // the S products, the conversion warps
         }
+#pragma unroll
+        for (int i = 0; i < kCstRing; ++i) pipe::mbar_init(&bars[G::kBarCst + i], kKeys / 32);
         pipe::mbar_init(&bars[G::kBarConv], G::kConvThreads);
         *gave_up = 0;
         *least = INT_MAX;
@@ -342,7 +350,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     const int j0 = static_cast<int>(static_cast<long long>(all_tiles) * blockIdx.z / gridDim.z);
     const int n_tiles = work ? static_cast<int>(static_cast<long long>(all_tiles) * (blockIdx.z + 1) / gridDim.z) - j0 : 0;
 
-    const int blk = warp < G::kSoftmaxWarps ? warp >> 3 : (warp < G::kConvWarp0 ? warp - G::kIssuerWarp0 : 0);
+    const int blk = warp < G::kSoftmaxWarps ? warp >> 3 : (warp > G::kIssuerWarp0 && warp < G::kConvWarp0 ? warp - G::kIssuerWarp0 - 1 : 0);
     const int wb = warp & 7;
     const int block_tok = blk * p.tokens_per_block;          // first token of the block, counted from token0
     uint64_t* const bb = bars + blk * G::kBarsPerBlock;
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         const int qpos_a = valid_a ? last_key(tok_a) : INT_MAX, qpos_b = valid_b ? last_key(tok_b) : INT_MAX;
         const float c_a = n_tiles > 0 ? row_amax[row_a] : 0.0f, c_b = n_tiles > 0 ? row_amax[row_b] : 0.0f;
         float m_a = kMInit, m_b = kMInit, l_a = 0.0f, l_b = 0.0f;
-        const float* const cst0 = reinterpret_cast<const float*>(sm + G::kSCst) + blk * kCstRing * G::kCstFloats;
+        const float* const cst0 = reinterpret_cast<const float*>(sm + G::kSCst);
         // One tile.  The plain form (kAny false) is for tiles that every row sees whole and whose V
         // scales are in the operand; kAny serves every tile.  Returns false when a wait gave up.
         auto weigh = [&](auto any, int i, const float* cst, int flags) -> bool {
@@ -480,8 +488,8 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                     f_a = f_b = 1.0f;
                 }
                 if (key0 + kKeys - 1 > seen_by_all || (flags & 15) != 15) {
-                    if (!wait_bar(&bars[G::kBarVReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word)) return false;   // marks of bad V rows
-                    const float* const poison = reinterpret_cast<const float*>(sm + G::kSPoison) + (i & 1) * kKeys + 2 * c2;
+                    if (!wait_bar(&bars[G::kBarVReady + i % kVBuffers], (i / kVBuffers) & 1, gave_up, __LINE__, p.error_word)) return false;   // marks of bad V rows
+                    const float* const poison = reinterpret_cast<const float*>(sm + G::kSPoison) + (i % kVBuffers) * kKeys + 2 * c2;
 #pragma unroll
                     for (int g = 0; g < 8; ++g) {
                         const int key = key0 + 8 * g + 2 * c2;
@@ -540,8 +548,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             }
             l_a += sum_a.x + sum_a.y;
             l_b += sum_b.x + sum_b.y;
-            // W buffer i % 2 is free: O += W_{i-2} V_{i-2} was issued before S_i by the same thread, and the commit that
-            // completed S_i's barrier covers it.  O may be touched once O += W_{i-1} V_{i-1} has completed; that wait may be
+            // W buffer i % 2 is free: the product thread arrives on S_i's barrier once O += W_{i-2} V_{i-2} is complete.  O may be touched once O += W_{i-1} V_{i-1} has completed; that wait may be
             // skipped on other tiles because no later product completes before this warp has signalled "W ready" for it.
             const bool rescale = moved && i > 0;
             if (rescale) {
@@ -632,68 +639,63 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         // =============================== products of row block `blk` ===============================
         constexpr uint32_t kIdescQK = instr_desc(kKeys, false);        // E4M3 operands have format number 0, as f16 has in its kind
         constexpr uint32_t kIdescPV = instr_desc(D, true);
-        const uint64_t q_hi = code_desc<D>(base + q_off), q_lo = code_desc<D>(base + q_off + G::kQPart);
-        const uint64_t k_tile = code_desc<D>(base + G::kSK), v_tile = smem_desc(base + G::kSV, kKeys * 128);
-        // S_t = hi K_t^T + lo K_t^T once K_t is there; the tile's constants go out with it, in the order of the weights
-        const int pos0 = ws::key_of_k_row(lane);             // the place of key `lane` (key 16 a + 8 h + 2 c + e lies at 16 a + 4 c + 2 h + e)
-        auto issue_qk = [&](int t) {
-            const int stage = t % kStages;
-            if (!wait_bar(&bars[G::kBarFull + stage], (t / kStages) & 1, gave_up, __LINE__, p.error_word)) return false;
-            tc_fence_after();
-            if (elect_one()) {
+        const uint64_t q_tile = code_desc<D>(base + G::kSQ), k_tile = code_desc<D>(base + G::kSK), v_tile = smem_desc(base + G::kSV, kKeys * 128);
+        // Whole warps walk the loops and one elected thread issues: loop counters, descriptors and tensor-memory addresses are
+        // then in uniform registers, where the instructions want them (in a branch of one thread each product costs about 130
+        // cycles of moves: 24 products a tile).  The two chains, S_{i+1} once S_i is read and O += W_i V_i once W_i is
+        // stored, are separate warps' so that neither waits for the other.
+        bool ok = true;
+        if (warp == G::kIssuerWarp0) {
+            for (int i = 0; i < n_tiles; ++i) {
+                const int stage = i % kStages;
                 const uint64_t kd = k_tile + static_cast<uint64_t>(stage * (G::kStageBytes >> 4));
+                ok = wait_bar(&bars[G::kBarFull + stage], (i / kStages) & 1, gave_up, __LINE__, p.error_word);
 #pragma unroll
-                for (int s = 0; s < D / 32; ++s) umma_f8(tmem_s, q_hi + 2 * s, kd + 2 * s, kIdescQK, s > 0);
+                for (int g = 0; g < kBlocks; ++g) {
+                    uint64_t* const of = bars + g * G::kBarsPerBlock;
+                    if (ok && i > 0) ok = wait_bar(&of[kBarSRead], (i - 1) & 1, gave_up, __LINE__, p.error_word);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t q_hi = q_tile + static_cast<uint64_t>(g * 2 * (G::kQPart >> 4)), q_lo = q_hi + (G::kQPart >> 4);
+                    const uint32_t d = tmem + g * kTmemCols;
+                    if (elect_one()) {
 #pragma unroll
-                for (int s = 0; s < D / 32; ++s) umma_f8(tmem_s, q_lo + 2 * s, kd + 2 * s, kIdescQK, true);
-                umma_commit(&bb[kBarQK + (t & 1)]);
-            }
-            const float* const ks = reinterpret_cast<const float*>(sm + G::kSK + stage * G::kStageBytes + G::kScaleAt);
-            float* const cst = reinterpret_cast<float*>(sm + G::kSCst) + (blk * kCstRing + (t & (kCstRing - 1))) * G::kCstFloats;
-            const int groups = stage_groups[stage], key0 = (j0 + t) * kKeys;
-            bool slow = false;
+                        for (int s = 0; s < D / 32; ++s) umma_f8(d, q_hi + 2 * s, kd + 2 * s, kIdescQK, s > 0);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key = lane + 32 * h;
-                cst[pos0 + 32 * h] = ks[key];
-                slow |= key0 + key < total_keys && ((groups >> (key >> 4)) & 1) && outside_fold(ks[kKeys + key]);
-            }
-            slow = __any_sync(0xffffffffu, slow);
-            if (slow) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float vs = ks[kKeys + lane + 32 * h];
-                    const float lg = fmaxf(lg2f(vs), kLgFloor) + static_cast<float>(kFoldShift);
-                    cst[kKeys + pos0 + 32 * h] = lg + vs * 0.0f;            // (the maximum loses a NaN scale: it is added back)
-                    cst[2 * kKeys + pos0 + 32 * h] = ex2f(-lg);
+                        for (int s = 0; s < D / 32; ++s) umma_f8(d, q_lo + 2 * s, kd + 2 * s, kIdescQK, true);
+                        umma_commit(&of[kBarQK + (i & 1)]);
+                        if (g == kBlocks - 1) umma_commit(&bars[G::kBarEmpty + stage]);        // K_i is free once these products are done
+                    }
+                    __syncwarp();
                 }
-            }
-            if (lane == 0) reinterpret_cast<int*>(cst)[3 * kKeys] = groups | (slow ? kSlow : 0);
-            __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bb[kBarQK + (t & 1)]);
-            return true;
-        };
-        bool ok = n_tiles > 0 && issue_qk(0);
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            if (i + 1 < n_tiles) {
-                ok = wait_bar(&bb[kBarSRead], i & 1, gave_up, __LINE__, p.error_word);
                 if (!ok) break;
-                if (lane == 0) pipe::mbar_arrive(&bars[G::kBarEmpty + i % kStages]);      // K_i's product is done, its scales are read
-                ok = issue_qk(i + 1);
-                if (!ok) break;
-            }
-            ok = wait_bar(&bb[kBarWReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word) &&
-                 wait_bar(&bars[G::kBarVReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint64_t vd = v_tile + static_cast<uint64_t>((i & 1) * (G::kTileBytes >> 4));
+                // what else tile i's scores need: its constants, and the W buffer that O += W_{i-2} V_{i-2} read
+                ok = wait_bar(&bars[G::kBarCst + (i & (kCstRing - 1))], (i / kCstRing) & 1, gave_up, __LINE__, p.error_word);
 #pragma unroll
-                for (int s = 0; s < kKeys / 16; ++s)
-                    umma_f16_ts(tmem_o, tmem_w + (i & 1) * (kKeys / 2) + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
-                umma_commit(&bb[kBarPV + (i & 1)]);
+                for (int g = 0; g < kBlocks; ++g) {
+                    uint64_t* const of = bars + g * G::kBarsPerBlock;
+                    if (ok && i >= 2) ok = wait_bar(&of[kBarPV + (i & 1)], ((i - 2) >> 1) & 1, gave_up, __LINE__, p.error_word);
+                    if (ok && lane == 0) pipe::mbar_arrive(&of[kBarQK + (i & 1)]);
+                }
+                if (!ok) break;
             }
-            __syncwarp();
+        } else {
+            for (int i = 0; i < n_tiles; ++i) {
+                const int buf = i % kVBuffers;
+                ok = wait_bar(&bars[G::kBarVReady + buf], (i / kVBuffers) & 1, gave_up, __LINE__, p.error_word) &&
+                     wait_bar(&bb[kBarWReady + (i & 1)], (i >> 1) & 1, gave_up, __LINE__, p.error_word);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t vd = v_tile + static_cast<uint64_t>(buf * (G::kTileBytes >> 4));
+                if (elect_one()) {
+#pragma unroll
+                    for (int s = 0; s < kKeys / 16; ++s)
+                        umma_f16_ts(tmem_o, tmem_w + (i & 1) * (kKeys / 2) + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
+                    umma_commit(&bb[kBarPV + (i & 1)]);
+                    umma_commit(&bars[G::kBarVEmpty + buf]);
+                }
+                __syncwarp();
+            }
         }
     } else if (warp < G::kCopyWarp) {
         // =============================== conversion of V ===============================
@@ -707,15 +709,12 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         };
         bool ok = true;
         for (int i = 0; i < n_tiles && ok; ++i) {
-            const int buf = i & 1, stage = i % kStages, key0 = (j0 + i) * kKeys;
+            const int buf = i % kVBuffers, stage = i % kStages, key0 = (j0 + i) * kKeys;
             const unsigned char* const raw = sm + G::kSK + stage * G::kStageBytes + G::kRawBytes;
             const float* const raw_vs = reinterpret_cast<const float*>(sm + G::kSK + stage * G::kStageBytes + G::kScaleAt) + kKeys;
             ok = wait_bar<50>(&bars[G::kBarFull + stage], (i / kStages) & 1, gave_up, __LINE__, p.error_word);
-            if (i >= 2) {        // the operand buffer is free once O += W_{i-2} V_{i-2} of every block is complete
-#pragma unroll
-                for (int g = 0; g < kBlocks; ++g)
-                    ok = ok && wait_bar<50>(&bars[g * G::kBarsPerBlock + kBarPV + buf], ((i - 2) >> 1) & 1, gave_up, __LINE__, p.error_word);
-            }
+            if (i >= kVBuffers)      // the operand buffer is free once every block's O += W V that read it is complete
+                ok = ok && wait_bar<50>(&bars[G::kBarVEmpty + buf], ((i / kVBuffers) - 1) & 1, gave_up, __LINE__, p.error_word);
             if (!ok) break;
             const int groups = stage_groups[stage];
             const bool edge = key0 + kKeys - 1 > seen_by_all || groups != 15;      // uniform
@@ -733,7 +732,23 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 if (!meet()) { ok = false; break; }
             }
             auto counts = [&](int k) { return key0 + k < total_keys && ((groups >> (k >> 4)) & 1) && outside_fold(raw_vs[k]); };
-            const bool slow = __any_sync(0xffffffffu, counts(lane) || counts(lane + 32));      // as the product warps decide
+            const bool slow = __any_sync(0xffffffffu, counts(lane) || counts(lane + 32));
+            if (t < kKeys) {
+                // the tile's constants, in the order of the weights (key 16 a + 8 h + 2 c + e lies at 16 a + 4 c + 2 h + e).  The slot's
+                // last reader was tile i - 4, which the softmax has left: O += W V of tile i - 3 is complete.
+                float* const cst = reinterpret_cast<float*>(sm + G::kSCst) + (i & (kCstRing - 1)) * G::kCstFloats;
+                const int place = ws::key_of_k_row(t);
+                cst[place] = raw_vs[t - kKeys];                                     // (the K scales lie in front of the V scales)
+                if (slow) {
+                    const float vs = raw_vs[t];
+                    const float lg = fmaxf(lg2f(vs), kLgFloor) + static_cast<float>(kFoldShift);
+                    cst[kKeys + place] = lg + vs * 0.0f;                            // (the maximum loses a NaN scale: it is added back)
+                    cst[2 * kKeys + place] = ex2f(-lg);
+                }
+                if (t == 0) reinterpret_cast<int*>(cst)[3 * kKeys] = groups | (slow ? kSlow : 0);
+                __syncwarp();
+                if (lane == 0) pipe::mbar_arrive(&bars[G::kBarCst + (i & (kCstRing - 1))]);
+            }
             // E4M3 -> f16 operand rows: [dim block of 64][row][128 bytes, swizzled].  Consecutive threads take consecutive
             // pieces of the raw tile; the upper half of a row's pieces stores its second half first, so that the eight
             // threads of a row write eight different 16-byte columns.
@@ -790,12 +805,10 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         };
         int id = page_of(0), next = page_of(1);
         int issued = 0;
-        bool ok = true;
-        for (int i = 0; i < n_tiles; ++i) {
+        auto copy_tile = [&](int i) {
             const int stage = i % kStages, after = page_of(i + 2);
             const unsigned have = __ballot_sync(0xffffffffu, id >= 0);               // the runs of the tile that exist
-            if (i >= kStages) ok = wait_bar<50>(&bars[G::kBarEmpty + stage], ((i / kStages) - 1) & 1, gave_up, __LINE__, p.error_word);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            if (i >= kStages && !wait_bar<50>(&bars[G::kBarEmpty + stage], ((i / kStages) - 1) & 1, gave_up, __LINE__, p.error_word)) return false;
             unsigned char* const dst = sm + G::kSK + stage * G::kStageBytes;
             uint64_t* const full = &bars[G::kBarFull + stage];
             if (elect_one()) {
@@ -806,7 +819,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 pipe::mbar_expect_tx(full, static_cast<uint32_t>((__popc(have) << run_shift) * 2 * D));
             }
             __syncwarp();
-            const int in_page = ((j0 + i) * kKeys) & ((1 << shift) - 1);             // (0 for pages of at most a tile)
+            const int in_page = ((j0 + i) * kKeys) & ((1 << shift) - 1) & ~(run_keys - 1);     // (0 for pages of at most a tile)
             for (int r = 0; r < runs; ++r) {
                 const int page = __shfl_sync(0xffffffffu, id, r);
                 if (page >= 0 && elect_one()) {
@@ -817,16 +830,17 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 }
                 __syncwarp();
             }
-            {
-                const int page = __shfl_sync(0xffffffffu, id, scale_key >> run_shift);
-                const size_t key = page >= 0 ? key_index(p.c, page, kvh) + in_page + (scale_key & (run_keys - 1)) : 0;
-                cp16_zfill(pipe::smem_u32(dst + G::kScaleAt + (lane >> 4) * (kKeys * 4) + scale_key * 4), scales + key, page >= 0);
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pipe::smem_u32(full)) : "memory");
-            }
+            const int page = __shfl_sync(0xffffffffu, id, scale_key >> run_shift);
+            const size_t key = page >= 0 ? key_index(p.c, page, kvh) + in_page + (scale_key & (run_keys - 1)) : 0;
+            cp16_zfill(pipe::smem_u32(dst + G::kScaleAt + (lane >> 4) * (kKeys * 4) + scale_key * 4), scales + key, page >= 0);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pipe::smem_u32(full)) : "memory");
             issued = i + 1;
             id = next;
             next = after;
-        }
+            return true;
+        };
+        bool ok = true;
+        for (int i = 0; i < n_tiles && ok; ++i) ok = copy_tile(i);
         if (!ok)        // somebody gave up: let the copies on their way land (bounded again) before the CTA ends
             for (int i = max(0, issued - kStages); i < issued; ++i)
                 for (int tries = 0; tries < (1 << 12) && !pipe::mbar_try_wait(&bars[G::kBarFull + i % kStages], (i / kStages) & 1); ++tries) {}
