@@ -130,7 +130,7 @@ struct Geo {
     static constexpr int kStageBytes = 2 * kRawBytes + 1024;
     static constexpr int kCstFloats = 3 * kKeys + 4;                        // K scales; where V scales ride in the exponent: log2, inverse; flags
     static constexpr int kSQ = 0;
-    static constexpr int kSK = kSQ + kBlocks * 2 * kQPart;
+    static constexpr int kSK = kSQ + kBlocks * kQPart;
     static constexpr int kSV = kSK + kStages * kStageBytes;
     static constexpr int kSRow = kSV + kVBuffers * kTileBytes;                    // per block: maxima of |q| (two halves of a row), then the rows' factors
     static constexpr int kSCst = kSRow + kBlocks * 2 * kRows * 4;           // [kCstRing]
@@ -174,6 +174,14 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// the same product with the rows (A) in tensor memory: lane = row, four codes per 32-bit column
+__device__ __forceinline__ void umma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
         : "memory");
 }
 // rows y .. of a [rows][D] byte array into shared memory, swizzled by the map; x is always 0
@@ -354,8 +362,9 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     const int wb = warp & 7;
     const int block_tok = blk * p.tokens_per_block;          // first token of the block, counted from token0
     uint64_t* const bb = bars + blk * G::kBarsPerBlock;
-    const uint32_t tmem_s = tmem + blk * kTmemCols, tmem_o = tmem_s + kKeys, tmem_w = tmem_o + kD;
-    const int q_off = G::kSQ + blk * 2 * G::kQPart;
+    const uint32_t tmem_s = tmem + blk * kTmemCols, tmem_o = tmem_s + kKeys, tmem_w = tmem_o + kD, tmem_q = tmem_w + kKeys / 2;
+    // a block's 256 columns: S 64, O 128, W 32 (f16 pairs), lo part of Q 32 (four codes each)
+    const int q_off = G::kSQ + blk * G::kQPart;
 
     // a row of a block: its head slot and token (counted from token0); whether it exists; the last key it sees
     auto row_at = [&](int row, int& tok, int& head) {
@@ -382,7 +391,8 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     }
     const int seen_by_all = kPrefix ? *least : held;
 
-    // ---- Q (softmax warps): bf16 -> two E4M3 parts in shared memory.  A row is scaled by a power of two so that its
+    // ---- Q (softmax warps): bf16 -> two E4M3 parts, hi in shared memory, lo in tensor memory (products whose rows come from
+    //      there read a third of the shared memory: its port is what this kernel fills first).  A row is scaled by a power of two so that its
     //      largest |q| lies in 2^7 .. 2^8; its scores take that back. ----
     float* const row_amax = reinterpret_cast<float*>(sm + G::kSRow) + blk * 2 * kRows;
     if (warp < G::kSoftmaxWarps && n_tiles > 0) {
@@ -413,22 +423,24 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         const bool finite = amax_a <= 3.4e38f && amax_b <= 3.4e38f;
         if (part == 0) row_amax[row] = finite ? fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23) : NAN;
         if (p.scale_log2e < 0.0f) down = -down;
+        uint32_t lo_words[4 * (kHalf / 2)];
 #pragma unroll
         for (int i = 0; i < kHalf / 2; ++i) {                // sixteen values: one 16-byte piece of each part
             const uint32_t words[8] = {w[2 * i].x, w[2 * i].y, w[2 * i].z, w[2 * i].w, w[2 * i + 1].x, w[2 * i + 1].y, w[2 * i + 1].z, w[2 * i + 1].w};
-            uint32_t hi[4], lo[4];
+            uint32_t hi[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 uint32_t h0, l0, h1, l1;
                 split_e4m3x2(bf_lo(words[2 * k]) * down, bf_hi(words[2 * k]) * down, h0, l0);
                 split_e4m3x2(bf_lo(words[2 * k + 1]) * down, bf_hi(words[2 * k + 1]) * down, h1, l1);
                 hi[k] = (h0 & 0xffffu) | (h1 << 16);
-                lo[k] = (l0 & 0xffffu) | (l1 << 16);
+                lo_words[4 * i + k] = (l0 & 0xffffu) | (l1 << 16);
             }
             const int at = q_off + code_at<D>(row, (kHalf / 2) * part + i);
             *reinterpret_cast<uint4*>(sm + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(sm + at + G::kQPart) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
+        tmem_st_words<4 * (kHalf / 2)>(tmem_q + (static_cast<uint32_t>(32 * (wb & 3)) << 16) + part * (4 * (kHalf / 2)), lo_words);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         fence_async_smem();
     }
     tc_fence_before();
@@ -548,15 +560,13 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             }
             l_a += sum_a.x + sum_a.y;
             l_b += sum_b.x + sum_b.y;
-            // W buffer i % 2 is free: the product thread arrives on S_i's barrier once O += W_{i-2} V_{i-2} is complete.  O may be touched once O += W_{i-1} V_{i-1} has completed; that wait may be
-            // skipped on other tiles because no later product completes before this warp has signalled "W ready" for it.
-            const bool rescale = moved && i > 0;
-            if (rescale) {
+            // W and O are free once O += W_{i-1} V_{i-1} is complete, a tile's work ago.
+            if (i > 0) {
                 if (!wait_bar(&bb[kBarPV + ((i - 1) & 1)], ((i - 1) >> 1) & 1, gave_up, __LINE__, p.error_word)) return false;
                 tc_fence_after();
             }
-            tmem_st_frag_x4(tmem_w + (i & 1) * (kKeys / 2) + my_lanes16, wv);
-            if (rescale) {
+            tmem_st_frag_x4(tmem_w + my_lanes16, wv);
+            if (moved && i > 0) {
                 const float2 ca = splat2(corr_a), cb2 = splat2(corr_b);
 #pragma unroll 1
                 for (int cb = 0; cb < D; cb += 64) {
@@ -656,27 +666,23 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                     if (ok && i > 0) ok = wait_bar(&of[kBarSRead], (i - 1) & 1, gave_up, __LINE__, p.error_word);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t q_hi = q_tile + static_cast<uint64_t>(g * 2 * (G::kQPart >> 4)), q_lo = q_hi + (G::kQPart >> 4);
-                    const uint32_t d = tmem + g * kTmemCols;
+                    const uint64_t q_hi = q_tile + static_cast<uint64_t>(g * (G::kQPart >> 4));
+                    const uint32_t d = tmem + g * kTmemCols, q_lo = d + kKeys + kD + kKeys / 2;
                     if (elect_one()) {
 #pragma unroll
                         for (int s = 0; s < D / 32; ++s) umma_f8(d, q_hi + 2 * s, kd + 2 * s, kIdescQK, s > 0);
 #pragma unroll
-                        for (int s = 0; s < D / 32; ++s) umma_f8(d, q_lo + 2 * s, kd + 2 * s, kIdescQK, true);
+                        for (int s = 0; s < D / 32; ++s) umma_f8_ts(d, q_lo + 8 * s, kd + 2 * s, kIdescQK, true);
                         umma_commit(&of[kBarQK + (i & 1)]);
                         if (g == kBlocks - 1) umma_commit(&bars[G::kBarEmpty + stage]);        // K_i is free once these products are done
                     }
                     __syncwarp();
                 }
                 if (!ok) break;
-                // what else tile i's scores need: its constants, and the W buffer that O += W_{i-2} V_{i-2} read
                 ok = wait_bar(&bars[G::kBarCst + (i & (kCstRing - 1))], (i / kCstRing) & 1, gave_up, __LINE__, p.error_word);
 #pragma unroll
-                for (int g = 0; g < kBlocks; ++g) {
-                    uint64_t* const of = bars + g * G::kBarsPerBlock;
-                    if (ok && i >= 2) ok = wait_bar(&of[kBarPV + (i & 1)], ((i - 2) >> 1) & 1, gave_up, __LINE__, p.error_word);
-                    if (ok && lane == 0) pipe::mbar_arrive(&of[kBarQK + (i & 1)]);
-                }
+                for (int g = 0; g < kBlocks; ++g)
+                    if (ok && lane == 0) pipe::mbar_arrive(&bars[g * G::kBarsPerBlock + kBarQK + (i & 1)]);      // the tile's constants are there
                 if (!ok) break;
             }
         } else {
@@ -690,7 +696,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 if (elect_one()) {
 #pragma unroll
                     for (int s = 0; s < kKeys / 16; ++s)
-                        umma_f16_ts(tmem_o, tmem_w + (i & 1) * (kKeys / 2) + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
+                        umma_f16_ts(tmem_o, tmem_w + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
                     umma_commit(&bb[kBarPV + (i & 1)]);
                     umma_commit(&bars[G::kBarVEmpty + buf]);
                 }
