@@ -190,6 +190,20 @@ __device__ __forceinline__ void tensor_load(void* dst, const CUtensorMap* map, i
                  "l"(map), "r"(0), "r"(y), "r"(pipe::smem_u32(bar))
                  : "memory");
 }
+// A value twice in a register pair, kept as one 64-bit operand: built from two floats at every use, a pair costs two moves
+// (a fifth of the softmax loop's instructions were these).
+__device__ __forceinline__ unsigned long long both(float v) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float2 fma2_both(float2 a, unsigned long long b, unsigned long long c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rd;\n\tmov.b64 ra, {%2, %3};\n\tfma.rn.f32x2 rd, ra, %4, %5;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "l"(b), "l"(c));
+    return d;
+}
 // true in one lane of the (whole) warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;
@@ -538,14 +552,14 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                 l_a *= corr_a;
                 l_b *= corr_b;
             }
-            const float2 f2_a = splat2(f_a), f2_b = splat2(f_b), neg_a = splat2(-m_a), neg_b = splat2(-m_b);
+            const unsigned long long f2_a = both(f_a), f2_b = both(f_b), neg_a = both(-m_a), neg_b = both(-m_b);
             float2 sum_a = make_float2(0.0f, 0.0f), sum_b = make_float2(0.0f, 0.0f);
             // word 4 (g / 2) + g % 2: row a, keys 8 g + 2 c2 + {0, 1}; + 2: row b.  In tensor memory that is pair 8 (g / 2) +
             // 2 c2 + g % 2 of the row, so V's rows are laid out in that order.
             uint32_t wv[16];
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
-                const float2 xa = fma2_rn(sv[2 * g], f2_a, neg_a), xb = fma2_rn(sv[2 * g + 1], f2_b, neg_b);
+                const float2 xa = fma2_both(sv[2 * g], f2_a, neg_a), xb = fma2_both(sv[2 * g + 1], f2_b, neg_b);
                 const float2 ea = make_float2(ex2f(xa.x), ex2f(xa.y)), eb = make_float2(ex2f(xb.x), ex2f(xb.y));
                 if (kAny && slow) {
                     const float2 rv = *reinterpret_cast<const float2*>(cst + 2 * kKeys + 16 * (g >> 1) + 4 * c2 + 2 * (g & 1));
