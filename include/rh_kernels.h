@@ -297,7 +297,7 @@ int rh_flash_prefill_packed_bf16(void* out, const void* q, long long q_stride, c
  *
  * partial: caller-owned scratch of rh_flash_decode_paged_scratch_floats(...) floats, 16-byte aligned; calls that may
  * overlap in time need one each.  num_seqs <= 4096.  Two kernels, three where the prefix
- * meets 65 or more query rows per kv head (it then runs on tcgen05); results do not depend on timing. */
+ * meets 17 or more query rows per kv head (it then runs on tcgen05); results do not depend on timing. */
 size_t rh_flash_decode_paged_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
 int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_stride, const rh_kv_pages* cache, int layer,
                                const int* rows_or_null, int num_seqs, int num_q_heads, float scale, float* partial,

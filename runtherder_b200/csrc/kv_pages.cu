@@ -576,6 +576,8 @@ int check_pages(const rh_kv_pages* c, const char* fn) {
                "%s: at most 2^24 pages, 1024 kv heads and 4096 layers", fn);
     RH_REQUIRE(static_cast<long long>(c->num_rows) * c->pages_per_row <= INT_MAX / 2 && static_cast<long long>(c->pages_per_row) * c->page_size <= INT_MAX / 2,
                RH_ERR_UNSUPPORTED_DIM, "%s: num_rows * pages_per_row and pages_per_row * page_size must stay below 2^30", fn);
+    RH_REQUIRE(static_cast<long long>(c->num_pages) * c->num_kv_heads * c->page_size <= INT_MAX, RH_ERR_UNSUPPORTED_DIM,
+               "%s: num_pages * num_kv_heads * page_size must stay below 2^31", fn);
     RH_REQUIRE(aligned16(c->k) && aligned16(c->v) && aligned16(c->k_scale) && aligned16(c->v_scale), RH_ERR_MISALIGNED,
                "%s: k, v, k_scale and v_scale must be 16-byte aligned", fn);
     return RH_OK;

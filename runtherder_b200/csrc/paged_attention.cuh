@@ -7,6 +7,7 @@
 #include <climits>
 
 #include "paged.cuh"
+#include "rh_pipeline.cuh"
 
 namespace rh {
 namespace paged {
@@ -16,9 +17,28 @@ constexpr float kMInit = -1.0e30f;    // m before any key (finite: differences s
 constexpr float kLgFloor = -100.0f;   // floor of log2(V scale): a zero scale must not give -inf - -inf
 constexpr int kMaxSeqs = 4096;        // sequences of a decode call
 constexpr int kOwnCols = 8;           // query heads of a segment of own keys
-constexpr int kPrefixCols = 16;       // query rows of a prefix segment
+constexpr int kPrefixCols = 8;        // query rows of a prefix segment
 constexpr int kHeaderInts = 4;        // {shared keys, own tiles per head, -, -}, then the first tile of every sequence
 constexpr int kSharedAlign = 256;     // the prefix is cut down to a multiple of this (the largest page), the rest is own
+
+// Bounded wait of a whole warp on an mbarrier phase: polls without the suspend-time hint (a hinted wait wakes late), the
+// lanes meet again behind it.  Returns false, for all lanes, when the phase never completed.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int where, int* error_word, int tries = 1 << 20) {
+    const uint32_t addr = pipe::smem_u32(bar);
+    for (int i = 0; i < tries; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (__all_sync(0xffffffffu, ok != 0)) return true;
+    }
+    if (error_word != nullptr) atomicCAS(error_word, 0, (where << 8) | 1);
+    return false;
+}
 
 struct DecodeArgs {
     Layer c;
@@ -55,16 +75,16 @@ __host__ __device__ constexpr int acc_offset(int cols) { return (2 * cols + 3) /
 __host__ __device__ constexpr long long state_floats(int cols, int dim) { return acc_offset(cols) + static_cast<long long>(cols) * dim; }
 
 // Warps of the grid that get tiles: at least kMinTilesPerWarp each where there are enough.
-constexpr int kMinTilesPerWarp = 2;
+constexpr int kMinTilesPerWarp = 4;
 __device__ __forceinline__ long long warps_in_use(long long total, long long warps) {
     const long long most = (total + kMinTilesPerWarp - 1) / kMinTilesPerWarp;
     return most < 1 ? 1 : (most < warps ? most : warps);
 }
 
-inline int decode_ctas() { return 3 * host::num_sms(); }
+inline int decode_ctas() { return 4 * host::num_sms(); }
 
 // Query rows per kv head (entries x group) from which the tensor-memory kernel takes the prefix.
-constexpr int kBlockRows = 65;
+constexpr int kBlockRows = 17;
 int prefix_splits(int num_seqs, int num_kv_heads, int group);
 
 struct DecodeScratch {

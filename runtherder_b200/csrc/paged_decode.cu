@@ -7,7 +7,7 @@
 // caller's scratch which a second kernel joins.  The reference decodes one sequence (flash_decode_split_bf16,
 // include/runtherder/kernels/flash_decode.cuh:27-62; flash_decode.cu here).
 //
-// Work.  A segment is (sequence, kv head, up to 8 query heads) for own keys and (kv head, 16 of the batch's query rows)
+// Work.  A segment is (sequence, kv head, up to 8 query heads) for own keys and (kv head, 8 of the batch's query rows)
 // for the prefix, cut into tiles of 16 keys.  All tiles of all segments form one line that is dealt out evenly to all
 // warps of the grid, so neither ragged lengths nor few long sequences leave SMs idle; a warp that crosses from one
 // segment into the next writes one state for each.  Segment s and warp w meet at most once and both only grow along
@@ -43,8 +43,11 @@ using tc::pack_f16x2;
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kTile = 16;              // keys per tile
-constexpr int kStages = 4;             // tiles in a warp's ring
-constexpr float kShift = 10.0f;        // weights enter the second product as 2^10 * weight: small ones stay normal in f16
+static_assert(kPrefixCols == 8 && kOwnCols == 8, "a segment has the eight columns of a product");
+constexpr int kStages = 3;             // tiles in a warp's ring
+constexpr int kDecCtas = 4;            // CTAs per SM
+constexpr float kLag = 8.0f;           // how far (log2) the running maximum may lie below the true one
+constexpr float kShift = 7.0f;         // weights enter the second product as 2^7 * weight (at most 2^15): small ones stay normal in f16
 
 // D(16x8, fp32) += A(16x16, f16, row) * B(16x8, f16, col)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -60,6 +63,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
+// 4-byte asynchronous copy; arrives on `bar` (which counts every lane) once it has landed
+__device__ __forceinline__ void cp4_arrive(void* dst, const void* src, uint64_t* bar) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(pipe::smem_u32(dst)), "l"(src) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(pipe::smem_u32(bar)) : "memory");
+}
+
 template <int D>
 struct Ring {
     static constexpr int kCodes = kTile * D;                         // bytes of K (or V) codes of a tile
@@ -70,8 +79,8 @@ struct Ring {
 };
 
 // One warp's way through `tiles` tiles of a segment: keys key0 .. key0 + 16 tiles - 1 of the list `pages`, of which the
-// first `limit` exist; kNT groups of eight columns.
-template <int D, int kNT>
+// first `limit` exist; eight columns (query rows).  Called by whole warps.
+template <int D>
 struct Walk {
     using R = Ring<D>;
     static constexpr int kKWords = D / 16;    // 32-bit words of a K row per lane = k-steps of the first product
@@ -81,174 +90,172 @@ struct Walk {
     const DecodeArgs& p;
     unsigned char* ring;
     uint64_t* full;
-    uint32_t& phase;          // tiles this warp has taken from its ring so far (the stage and parity of the next one)
+    uint32_t& turn;           // tiles this warp has taken from its ring so far, modulo 2 kStages: stage and parity of the next
     int lane, r, c;
 
-    float o[kNT][kMB][4];
-    float m[kNT][2], l[kNT][2];
+    float o[kMB][4];
+    float m[2], l[2];         // of columns 2c and 2c + 1; l: this lane's part
 
-    __device__ __forceinline__ Walk(const DecodeArgs& p_, unsigned char* ring_, uint64_t* full_, uint32_t& phase_)
-        : p(p_), ring(ring_), full(full_), phase(phase_) {
+    __device__ __forceinline__ Walk(const DecodeArgs& p_, unsigned char* ring_, uint64_t* full_, uint32_t& turn_)
+        : p(p_), ring(ring_), full(full_), turn(turn_) {
         lane = threadIdx.x & 31;
         r = lane >> 2;
         c = lane & 3;
     }
 
-    // col_row(col): query row (in units of head_dim) of a column, -1: none; col_limit(col): keys that the column sees.
+    // col_row(col): offset of a column's query row, -1: none; col_limit(col): keys that the column sees.
     // Returns false when a wait gave up.
     template <typename ColRow, typename ColLimit>
     __device__ __forceinline__ bool run(const int* pages, int columns, int key0, int tiles, int limit, int kvh, ColRow col_row, ColLimit col_limit) {
-        const int shift = p.c.page_shift;
-        // ids of the pages of the next 32 tiles, one per lane; -1 where there is no page
-        auto fetch_ids = [&](int first) {
+        const int shift = p.c.page_shift, per_page = shift - 4;
+        // where the next 32 tiles lie, one per lane, in units of tiles from the start of the layer; -1 where there is no page
+        auto places = [&](int first) {
             const int key = key0 + (first + lane) * kTile;
             int id = -1;
             if (first + lane < tiles && (key >> shift) < columns) id = pages[key >> shift];
-            return id >= 0 && id < p.c.num_pages ? id : -1;
+            return id >= 0 && id < p.c.num_pages ? ((id * p.c.num_kv_heads + kvh) << per_page) + ((key >> 4) & ((1 << per_page) - 1)) : -1;
         };
-        int ids = fetch_ids(0), ids_next = fetch_ids(32);
-        auto issue = [&](int i, int id) {       // warp-uniform; a tile without a page takes its turn without bytes
-            const uint32_t at = phase + static_cast<uint32_t>(i);
-            const int stage = at % kStages;
+        int here = places(0), ahead = places(32);
+        uint32_t live = 0;                      // bit i % 32: tile i has a page
+        uint32_t put = turn;                    // the stage that is filled next
+        auto issue = [&](int i) {               // a tile without a page takes its turn without bytes
+            const int at = __shfl_sync(0xffffffffu, here, i & 31);
+            if ((i & 31) == 31) {
+                here = ahead;
+                ahead = places(i + 33);
+            }
+            const uint32_t stage = put >= kStages ? put - kStages : put;
+            put = put + 1 == 2 * kStages ? 0 : put + 1;
+            uint64_t* const bar = full + stage;
+            unsigned char* const dst = ring + stage * R::kStageBytes;
+            const bool there = at >= 0;
+            live = there ? live | (1u << (i & 31)) : live & ~(1u << (i & 31));
+            const size_t tile = there ? static_cast<size_t>(at) : 0;
             if (lane == 0) {
-                uint64_t* const bar = full + stage;
-                if (id >= 0) {
-                    unsigned char* const dst = ring + stage * R::kStageBytes;
-                    const size_t key = key_index(p.c, id, kvh) + ((key0 + i * kTile) & ((1 << shift) - 1));
-                    pipe::mbar_expect_tx(bar, R::kStageBytes);
-                    pipe::bulk_load(dst, p.c.k + key * D, R::kCodes, bar);
-                    pipe::bulk_load(dst + R::kCodes, p.c.v + key * D, R::kCodes, bar);
-                    pipe::bulk_load(dst + 2 * R::kCodes, p.c.k_scale + key, kTile * 4, bar);
-                    pipe::bulk_load(dst + 2 * R::kCodes + kTile * 4, p.c.v_scale + key, kTile * 4, bar);
+                if (there) {
+                    pipe::mbar_expect_tx(bar, 2 * R::kCodes);
+                    pipe::bulk_load(dst, p.c.k + tile * R::kCodes, R::kCodes, bar);
+                    pipe::bulk_load(dst + R::kCodes, p.c.v + tile * R::kCodes, R::kCodes, bar);
                 } else {
                     pipe::mbar_arrive(bar);
                 }
             }
-        };
-        auto id_of = [&](int i, int base) {     // tile i's page, from the lists that start at tile `base` and base + 32
-            const int a = __shfl_sync(0xffffffffu, ids, (i - base) & 31), b = __shfl_sync(0xffffffffu, ids_next, (i - base) & 31);
-            return i - base < 32 ? a : b;
+            // the scales: one per lane (K, then V), by ordinary asynchronous copies that arrive on the same barrier
+            cp4_arrive(dst + 2 * R::kCodes + lane * 4, (lane < kTile ? p.c.k_scale : p.c.v_scale) + tile * kTile + (lane & (kTile - 1)), bar);
         };
         __syncwarp();                           // the ring's last readers are done
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i)
-            if (i < tiles) issue(i, id_of(i, 0));
+#pragma unroll 1
+        for (int i = 0; i < min(kStages - 1, tiles); ++i) issue(i);
 
-        // ---- q as the B operand: column r of each group, dims 64 ch + 16 c + 0..15, scaled by a power of two into
-        //      (-2, 2) (exact; f16 then holds any bf16 row) ----
-        uint32_t qb[kNT][kKWords][2];
-        float factor[kNT][2];
-        int see[kNT][2];      // keys that the columns 2c and 2c + 1 see
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-            const long long row = col_row(8 * nt + r);
-            float qf[D / 4];
+        // ---- q as the B operand: column r, dims 64 ch + 16 c + 0..15, scaled by a power of two into (-2, 2) (exact; f16 then
+        //      holds any bf16 row) ----
+        uint32_t qb[kKWords][2];
+        float factor[2];
+        int see[2];                             // keys that the columns 2c and 2c + 1 see
+        {
+            const long long row = col_row(r);
+            uint4 raw[D / 32];
 #pragma unroll
             for (int ch = 0; ch < D / 64; ++ch) {
-                uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+                raw[2 * ch] = raw[2 * ch + 1] = make_uint4(0u, 0u, 0u, 0u);
                 if (row >= 0) {
                     const uint4* const src = reinterpret_cast<const uint4*>(p.q + row + 64 * ch + 16 * c);
-                    a = src[0];
-                    b = src[1];
+                    raw[2 * ch] = src[0];
+                    raw[2 * ch + 1] = src[1];
                 }
-                float f[8];
-                unpack8(a, f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) qf[16 * ch + i] = f[i];
-                unpack8(b, f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) qf[16 * ch + 8 + i] = f[i];
             }
-            float amax = 0.0f;
+            const int sees = min(limit, col_limit(r));
+            see[0] = __shfl_sync(0xffffffffu, sees, 8 * c);
+            see[1] = __shfl_sync(0xffffffffu, sees, 8 * c + 4);
+            uint32_t amax2 = 0u;
 #pragma unroll
-            for (int i = 0; i < D / 4; ++i) amax = fmaxf(amax, fabsf(qf[i]));
+            for (int v = 0; v < D / 32; ++v) amax2 = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax2, raw[v].x), raw[v].y), raw[v].z), raw[v].w);
+            float amax = fmaxf(bf_lo(amax2), bf_hi(amax2));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
             e = amax > 0.0f ? max(-100, min(126, e)) : 0;
             const float down = __int_as_float((127 - e) << 23);
             const float mine = p.scale_log2e * __int_as_float((127 + e) << 23);
-            factor[nt][0] = __shfl_sync(0xffffffffu, mine, 8 * c);
-            factor[nt][1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
-            const int sees = min(limit, col_limit(8 * nt + r));
-            see[nt][0] = __shfl_sync(0xffffffffu, sees, 8 * c);
-            see[nt][1] = __shfl_sync(0xffffffffu, sees, 8 * c + 4);
+            factor[0] = __shfl_sync(0xffffffffu, mine, 8 * c);
+            factor[1] = __shfl_sync(0xffffffffu, mine, 8 * c + 4);
 #pragma unroll
             for (int s = 0; s < kKWords; ++s) {
-                qb[nt][s][0] = pack_f16x2(qf[4 * s] * down, qf[4 * s + 1] * down);
-                qb[nt][s][1] = pack_f16x2(qf[4 * s + 2] * down, qf[4 * s + 3] * down);
+                const uint4& w = raw[s >> 1];
+                const uint32_t lo = s & 1 ? w.z : w.x, hi = s & 1 ? w.w : w.y;
+                qb[s][0] = pack_f16x2(bf_lo(lo) * down, bf_hi(lo) * down);
+                qb[s][1] = pack_f16x2(bf_lo(hi) * down, bf_hi(hi) * down);
             }
         }
-        int everyone = INT_MAX;      // keys that every column of the warp sees
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) everyone = min(everyone, min(see[nt][0], see[nt][1]));
-        everyone = __reduce_min_sync(0xffffffffu, everyone);
+        // tiles that every column sees whole
+        const int everyone = __reduce_min_sync(0xffffffffu, min(see[0], see[1]));
+        const int plain = max(0, min(tiles, (everyone - key0) >> 4));
 
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-            for (int b = 0; b < kMB; ++b) o[nt][b][0] = o[nt][b][1] = o[nt][b][2] = o[nt][b][3] = 0.0f;
-            m[nt][0] = m[nt][1] = kMInit;
-            l[nt][0] = l[nt][1] = 0.0f;
-        }
+        for (int b = 0; b < kMB; ++b) o[b][0] = o[b][1] = o[b][2] = o[b][3] = 0.0f;
+        m[0] = m[1] = kMInit;
+        l[0] = l[1] = 0.0f;
 
-        const int key_a = 4 * (r >> 1) + (r & 1);      // tile-local keys of rows r and r + 8 of the first product
-        int base = 0;
         bool ok = true;
+#pragma unroll 1
         for (int i = 0; i < tiles; ++i) {
-            if (i - base == 32) {
-                base += 32;
-                ids = ids_next;
-                ids_next = fetch_ids(base + 32);
-            }
             __syncwarp();                              // the stage that is filled next has been read by every lane
-            if (i + kStages - 1 < tiles) issue(i + kStages - 1, id_of(i + kStages - 1, base));
-            const int id = id_of(i, base);
-            const uint32_t at = phase + static_cast<uint32_t>(i);
-            const int stage = at % kStages;
-            ok = pipe::mbar_wait(full + stage, (at / kStages) & 1, __LINE__, p.error_word);
-            if (!__all_sync(0xffffffffu, ok)) {        // gave up: let the copies on their way land (bounded again), then leave
-                for (int k = 1; k < kStages && i + k < tiles; ++k)
-                    (void)pipe::mbar_wait(full + (at + k) % kStages, ((at + k) / kStages) & 1, __LINE__, p.error_word, 64);
-                ok = false;
+            if (i + kStages - 1 < tiles) issue(i + kStages - 1);
+            const uint32_t stage = turn >= kStages ? turn - kStages : turn;
+            ok = warp_wait(full + stage, turn >= kStages ? 1 : 0, __LINE__, p.error_word);
+            if (!ok) {                                 // gave up: let the copies on their way land (bounded again), then leave
+                for (int k = 1; k < kStages && i + k < tiles; ++k) {
+                    const uint32_t t = (turn + k) % (2 * kStages);
+                    (void)warp_wait(full + t % kStages, t >= kStages ? 1 : 0, __LINE__, p.error_word, 1 << 12);
+                }
                 break;
             }
-            if (id >= 0) fold(ring + stage * R::kStageBytes, key0 + i * kTile, key_a, qb, factor, see, everyone);
+            turn = turn + 1 == 2 * kStages ? 0 : turn + 1;
+            if ((live >> (i & 31)) & 1u) {
+                if (i < plain) fold<false>(ring + stage * R::kStageBytes, key0 + i * kTile, qb, factor, see);
+                else fold<true>(ring + stage * R::kStageBytes, key0 + i * kTile, qb, factor, see);
+            }
         }
-        phase += static_cast<uint32_t>(tiles);
         return ok;
     }
 
-    __device__ __forceinline__ void fold(const unsigned char* st, int kb, int key_a, const uint32_t (&qb)[kNT][kKWords][2],
-                                         const float (&factor)[kNT][2], const int (&see)[kNT][2], int everyone) {
-        // ---- this lane's part of the tile ----
-        uint32_t kw[2][kKWords], vw[4][kVWords];
+    // kPartial: some column must not see some of the tile's keys.
+    template <bool kPartial>
+    __device__ __forceinline__ void fold(const unsigned char* st, int kb, const uint32_t (&qb)[kKWords][2], const float (&factor)[2], const int (&see)[2]) {
+        const int key_a = 4 * (r >> 1) + (r & 1);      // tile-local keys of rows r and r + 8 of the first product: key_a, key_a + 2
+        // ---- S^T = K q^T ----
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int ch = 0; ch < D / 64; ++ch) {
+            const uint4 ka = *reinterpret_cast<const uint4*>(st + key_a * D + 64 * ch + 16 * c);
+            const uint4 kc = *reinterpret_cast<const uint4*>(st + (key_a + 2) * D + 64 * ch + 16 * c);
+            const uint32_t aw[4] = {ka.x, ka.y, ka.z, ka.w}, bw[4] = {kc.x, kc.y, kc.z, kc.w};
 #pragma unroll
-            for (int ch = 0; ch < D / 64; ++ch) {
-                const uint4 t = *reinterpret_cast<const uint4*>(st + (key_a + 2 * j) * D + 64 * ch + 16 * c);
-                kw[j][4 * ch] = t.x; kw[j][4 * ch + 1] = t.y; kw[j][4 * ch + 2] = t.z; kw[j][4 * ch + 3] = t.w;
+            for (int k = 0; k < 4; ++k) {
+                uint32_t a0, a1, a2, a3;
+                e4m3x4_to_f16x2x2(aw[k], a0, a2);
+                e4m3x4_to_f16x2x2(bw[k], a1, a3);
+                mma16816(k & 1 ? t : s, a0, a1, a2, a3, qb[4 * ch + k][0], qb[4 * ch + k][1]);
             }
+        }
+        uint32_t vw[4][kVWords];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const unsigned char* const src = st + R::kCodes + (4 * c + i) * D + r * (D / 8);
             if constexpr (D == 128) {
-                const uint4 t = *reinterpret_cast<const uint4*>(src);
-                vw[i][0] = t.x; vw[i][1] = t.y; vw[i][2] = t.z; vw[i][3] = t.w;
+                const uint4 v = *reinterpret_cast<const uint4*>(src);
+                vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
             } else {
-                const uint2 t = *reinterpret_cast<const uint2*>(src);
-                vw[i][0] = t.x; vw[i][1] = t.y;
+                const uint2 v = *reinterpret_cast<const uint2*>(src);
+                vw[i][0] = v.x; vw[i][1] = v.y;
             }
         }
-        const float* const sc = reinterpret_cast<const float*>(st + 2 * R::kCodes);
-        const float ks_a = sc[key_a], ks_b = sc[key_a + 2];
-        const float lg_a = fmaxf(lg2f(sc[kTile + key_a]), kLgFloor), lg_b = fmaxf(lg2f(sc[kTile + key_a + 2]), kLgFloor);
-        // NaN scales must reach the result: fmaxf drops a NaN, so it is added back
-        float nan_a = sc[kTile + key_a] * 0.0f, nan_b = sc[kTile + key_a + 2] * 0.0f;
+        const float* const sc = reinterpret_cast<const float*>(st + 2 * R::kCodes) + key_a;
+        const float ks_a = sc[0], ks_b = sc[2], vs_a = sc[kTile], vs_b = sc[kTile + 2];
+        const float lg_a = fmaxf(lg2f(vs_a), kLgFloor), lg_b = fmaxf(lg2f(vs_b), kLgFloor);
         const float rv_a = ex2f(-lg_a - kShift), rv_b = ex2f(-lg_b - kShift);
-        const bool partial = kb + kTile > everyone;
-        if (partial) {
+        float add_a = fmaf(vs_a, 0.0f, lg_a), add_b = fmaf(vs_b, 0.0f, lg_b);        // (the maximum loses a NaN scale: it is added back)
+        if constexpr (kPartial) {
             // A column must not see some of these keys, whose V codes may be anything: a NaN code times weight zero would
             // be NaN.  NaN codes become zero here, and the score of such a key NaN for the columns that do see it.
             unsigned bad[4];
@@ -264,98 +271,81 @@ struct Walk {
                 bad[i] = __ballot_sync(0xffffffffu, nan);
             }
             const unsigned lanes = 0x11111111u << (r >> 1);      // the lanes that hold key_a's and key_b's V rows
-            if (((r & 1) ? bad[1] : bad[0]) & lanes) nan_a = NAN;
-            if (((r & 1) ? bad[3] : bad[2]) & lanes) nan_b = NAN;
+            if (((r & 1) ? bad[1] : bad[0]) & lanes) add_a = NAN;
+            if (((r & 1) ? bad[3] : bad[2]) & lanes) add_b = NAN;
         }
-        // ---- S^T = K q^T ----
-        float s[kNT][4];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kKWords; ++k) {
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_to_f16x2x2(kw[0][k], a0, a2);
-            e4m3x4_to_f16x2x2(kw[1][k], a1, a3);
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qb[nt][k][0], qb[nt][k][1]);
+        // log2-domain scores with the V scale in the exponent: rows a, b x columns 2c, 2c + 1
+        float x0 = fmaf(s[0] + t[0], ks_a * factor[0], add_a), x1 = fmaf(s[1] + t[1], ks_a * factor[1], add_a);
+        float x2 = fmaf(s[2] + t[2], ks_b * factor[0], add_b), x3 = fmaf(s[3] + t[3], ks_b * factor[1], add_b);
+        if constexpr (kPartial) {
+            if (kb + key_a >= see[0]) x0 = -INFINITY;
+            if (kb + key_a >= see[1]) x1 = -INFINITY;
+            if (kb + key_a + 2 >= see[0]) x2 = -INFINITY;
+            if (kb + key_a + 2 >= see[1]) x3 = -INFINITY;
         }
-        uint32_t b0[kNT], b1[kNT];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-            // log2-domain scores with the V scale in the exponent: rows a, b x columns 2c, 2c + 1
-            float x0 = fmaf(s[nt][0], ks_a * factor[nt][0], lg_a) + nan_a, x1 = fmaf(s[nt][1], ks_a * factor[nt][1], lg_a) + nan_a;
-            float x2 = fmaf(s[nt][2], ks_b * factor[nt][0], lg_b) + nan_b, x3 = fmaf(s[nt][3], ks_b * factor[nt][1], lg_b) + nan_b;
-            if (partial) {
-                if (kb + key_a >= see[nt][0]) x0 = -INFINITY;
-                if (kb + key_a >= see[nt][1]) x1 = -INFINITY;
-                if (kb + key_a + 2 >= see[nt][0]) x2 = -INFINITY;
-                if (kb + key_a + 2 >= see[nt][1]) x3 = -INFINITY;
-            }
-            float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+        // The maximum may lag the true one by up to 2^kLag, so the eight rows need not agree on it on most tiles.
+        float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+        if (__any_sync(0xffffffffu, t0 > m[0] + kLag || t1 > m[1] + kLag)) {
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) {
                 t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
                 t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
             }
-            const float n0 = fmaxf(m[nt][0], t0), n1 = fmaxf(m[nt][1], t1);
-            if (__any_sync(0xffffffffu, n0 != m[nt][0] || n1 != m[nt][1])) {
-                const float f0 = ex2f(m[nt][0] - n0), f1 = ex2f(m[nt][1] - n1);
-                l[nt][0] *= f0;
-                l[nt][1] *= f1;
+            const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
+            const float f0 = ex2f(m[0] - n0), f1 = ex2f(m[1] - n1);
+            l[0] *= f0;
+            l[1] *= f1;
 #pragma unroll
-                for (int b = 0; b < kMB; ++b) {
-                    o[nt][b][0] *= f0; o[nt][b][1] *= f1;
-                    o[nt][b][2] *= f0; o[nt][b][3] *= f1;
-                }
-                m[nt][0] = n0;
-                m[nt][1] = n1;
+            for (int b = 0; b < kMB; ++b) {
+                o[b][0] *= f0; o[b][1] *= f1;
+                o[b][2] *= f0; o[b][3] *= f1;
             }
-            const float w0 = ex2f(x0 - n0 + kShift), w1 = ex2f(x1 - n1 + kShift), w2 = ex2f(x2 - n0 + kShift), w3 = ex2f(x3 - n1 + kShift);
-            // a masked key adds nothing to the denominator even where its stale V scale is no number
-            l[nt][0] += (w0 == 0.0f ? 0.0f : w0 * rv_a) + (w2 == 0.0f ? 0.0f : w2 * rv_b);
-            l[nt][1] += (w1 == 0.0f ? 0.0f : w1 * rv_a) + (w3 == 0.0f ? 0.0f : w3 * rv_b);
-            b0[nt] = transpose8x8(pack_f16x2(w0, w1));
-            b1[nt] = transpose8x8(pack_f16x2(w2, w3));
+            m[0] = n0;
+            m[1] = n1;
         }
+        const float s0 = m[0] - kShift, s1 = m[1] - kShift;
+        const float w0 = ex2f(x0 - s0), w1 = ex2f(x1 - s1), w2 = ex2f(x2 - s0), w3 = ex2f(x3 - s1);
+        if constexpr (kPartial) {       // a masked key adds nothing to the denominator even where its stale V scale is no number
+            l[0] += (w0 == 0.0f ? 0.0f : w0 * rv_a) + (w2 == 0.0f ? 0.0f : w2 * rv_b);
+            l[1] += (w1 == 0.0f ? 0.0f : w1 * rv_a) + (w3 == 0.0f ? 0.0f : w3 * rv_b);
+        } else {
+            l[0] = fmaf(w2, rv_b, fmaf(w0, rv_a, l[0]));
+            l[1] = fmaf(w3, rv_b, fmaf(w1, rv_a, l[1]));
+        }
+        const uint32_t b0 = transpose8x8(pack_f16x2(w0, w1)), b1 = transpose8x8(pack_f16x2(w2, w3));
         // ---- O^T += V^T W^T: bytes of keys 4c .. 4c + 3 transposed into key pairs ----
 #pragma unroll
         for (int w = 0; w < kVWords; ++w) {
             const uint32_t t01 = __byte_perm(vw[0][w], vw[1][w], 0x5140), t23 = __byte_perm(vw[2][w], vw[3][w], 0x5140);
             const uint32_t u01 = __byte_perm(vw[0][w], vw[1][w], 0x7362), u23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
-            uint32_t a0, a1, a2, a3, e0, e1, e2, e3;
+            uint32_t a0, a1, a2, a3;
             e4m3x4_to_f16x2x2(t01, a0, a1);
             e4m3x4_to_f16x2x2(t23, a2, a3);
-            e4m3x4_to_f16x2x2(u01, e0, e1);
-            e4m3x4_to_f16x2x2(u23, e2, e3);
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-                mma16816(o[nt][2 * w], a0, a1, a2, a3, b0[nt], b1[nt]);
-                mma16816(o[nt][2 * w + 1], e0, e1, e2, e3, b0[nt], b1[nt]);
-            }
+            mma16816(o[2 * w], a0, a1, a2, a3, b0, b1);
+            e4m3x4_to_f16x2x2(u01, a0, a1);
+            e4m3x4_to_f16x2x2(u23, a2, a3);
+            mma16816(o[2 * w + 1], a0, a1, a2, a3, b0, b1);
         }
     }
 
     // The state of the columns < live to `slot`: m [cols], l [cols], acc [cols][D] (cols: the slot's columns)
-    __device__ __forceinline__ void store(float* slot, int cols, int live) {
+    __device__ __forceinline__ void store(float* slot, int cols, int used) {
         const float unshift = ex2f(-kShift);
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float sum = l[nt][e];
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                const int col = 8 * nt + 2 * c + e;
-                if (col < live) {
-                    if (r == 0) {
-                        slot[col] = m[nt][e];
-                        slot[cols + col] = sum;
-                    }
-                    float4* const dst = reinterpret_cast<float4*>(slot + acc_offset(cols) + col * D + r * (D / 8));
-#pragma unroll
-                    for (int q = 0; q < kMB / 2; ++q)
-                        dst[q] = make_float4(o[nt][2 * q][e] * unshift, o[nt][2 * q][2 + e] * unshift, o[nt][2 * q + 1][e] * unshift, o[nt][2 * q + 1][2 + e] * unshift);
+            for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            const int col = 2 * c + e;
+            if (col < used) {
+                if (r == 0) {
+                    slot[col] = m[e];
+                    slot[cols + col] = sum;
                 }
+                float4* const dst = reinterpret_cast<float4*>(slot + acc_offset(cols) + col * D + r * (D / 8));
+#pragma unroll
+                for (int q = 0; q < kMB / 2; ++q)
+                    dst[q] = make_float4(o[2 * q][e] * unshift, o[2 * q][2 + e] * unshift, o[2 * q + 1][e] * unshift, o[2 * q + 1][2 + e] * unshift);
             }
         }
     }
@@ -372,14 +362,14 @@ __device__ __forceinline__ int keys_of(const DecodeArgs& p, int b) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kDecThreads, 3) decode_kernel(const DecodeArgs p) {
+__global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(const DecodeArgs p) {
     using R = Ring<D>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int warp_sum[kDecWarps];
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + R::kBarOffset);
     int* const first_tile = reinterpret_cast<int*>(smem + R::kTableOffset);     // [num_seqs + 1], in tiles of one kv head
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x < kDecWarps * kStages) pipe::mbar_init(bars + threadIdx.x, 1);
+    if (threadIdx.x < kDecWarps * kStages) pipe::mbar_init(bars + threadIdx.x, 1 + 32);      // the codes' bytes, and every lane's scale
     pipe::mbar_init_fence();
 
     pdl_wait();
@@ -431,7 +421,7 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_kernel(const DecodeArgs
 
     unsigned char* const ring = smem + warp * R::kWarpBytes;
     uint64_t* const full = bars + warp * kStages;
-    uint32_t phase = 0;
+    uint32_t turn = 0;
     bool ok = true;
     while (t < end && ok) {
         if (t < prefix_total) {
@@ -439,7 +429,7 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_kernel(const DecodeArgs
             const int tiles = static_cast<int>(min(end - t, static_cast<long long>(prefix_tiles - at)));
             const int kvh = seg / p.prefix_chunks, row0 = (seg - kvh * p.prefix_chunks) * kPrefixCols;
             const int rows = p.num_seqs * p.group;
-            Walk<D, 2> walk(p, ring, full, phase);
+            Walk<D> walk(p, ring, full, turn);
             ok = walk.run(p.shared_pages, p.c.pages_per_row, at * kTile, tiles, shared_keys, kvh,
                           [&](int col) -> long long {
                               const int row = row0 + col;
@@ -467,7 +457,7 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_kernel(const DecodeArgs
             const int row = p.rows != nullptr ? p.rows[b] : b;
             const int live = min(p.own_cols, p.group - h0);
             const int keys = keys_of(p, b);
-            Walk<D, 1> walk(p, ring, full, phase);
+            Walk<D> walk(p, ring, full, turn);
             ok = walk.run(p.c.page_table + static_cast<size_t>(row) * p.c.pages_per_row, p.c.pages_per_row, shared_keys + at * kTile, tiles, keys, kvh,
                           [&](int col) -> long long { return col < live ? b * p.q_stride + static_cast<long long>(kvh * p.group + h0 + col) * D : -1; },
                           [&](int) { return keys; });
@@ -481,7 +471,7 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_kernel(const DecodeArgs
 // was seen.  kRowThreads threads share a row: D / 4 lanes hold four dims each, the groups of lanes take the states in
 // turn.  A whole CTA per row where there are few rows (a lone sequence has as many states as warps worked on it), a
 // few lanes where there are many.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 1024;
 
 template <int D, int kRowThreads>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs p, long long decode_warps) {

@@ -291,6 +291,13 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     // (through a shuffle, so that the compiler knows the warp's number and what follows from it to be uniform: the product
     // warps' descriptors then live in uniform registers)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if constexpr (kPrefix) {
+        if (*p.shared_len < kSharedAlign) {      // nothing is shared: no state is written, and none is read
+            pdl_trigger();
+            pdl_wait();
+            return;
+        }
+    }
     const int kvh = blockIdx.x / p.head_chunks;
     const int chunk = blockIdx.x - kvh * p.head_chunks;
 
@@ -934,7 +941,6 @@ int make_k_map(const Layer& c, int head_dim, const char* fn, CUtensorMap* map) {
     }();
     RH_REQUIRE(encode != nullptr, RH_ERR_CUDA, "%s: the driver has no cuTensorMapEncodeTiled", fn);
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), (static_cast<cuuint64_t>(c.num_pages) * c.num_kv_heads) << c.page_shift};
-    RH_REQUIRE(dims[1] <= INT_MAX, RH_ERR_UNSUPPORTED_DIM, "%s: a layer must hold fewer than 2^31 keys x kv heads", fn);
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim)};
     const int page = 1 << c.page_shift;
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(head_dim), static_cast<cuuint32_t>(page < kKeys ? page : kKeys)}, steps[2] = {1, 1};

@@ -36,7 +36,7 @@ def append(cache, layer=0, k=A, v=A, ks=256, vs=256, rows=None, cu=A, tokens=4, 
     (dict(num_pages=0), INVALID), (dict(num_rows=-1), INVALID), (dict(pages_per_row=0), INVALID), (dict(num_kv_heads=0), INVALID),
     (dict(page_size=8), DIM), (dict(page_size=24), DIM), (dict(page_size=512), DIM), (dict(page_size=0), DIM), (dict(head_dim=96), DIM),
     (dict(head_dim=256), DIM), (dict(num_pages=1 << 25), DIM), (dict(num_rows=1 << 20, pages_per_row=1 << 12), DIM),
-    (dict(k=A + 8), MISALIGNED), (dict(v_scale=A + 4), MISALIGNED),
+    (dict(num_pages=1 << 23, num_kv_heads=8, page_size=64), DIM), (dict(k=A + 8), MISALIGNED), (dict(v_scale=A + 4), MISALIGNED),
 ])
 def test_bad_cache_descriptions(change, want):
     c = pages(**change)
