@@ -469,24 +469,22 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(const Dec
 
 // Joins the states of a query row: M = max m_i, out = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i, zero where nothing
 // was seen.  kRowThreads threads share a row: D / 4 lanes hold four dims each, the groups of lanes take the states in
-// turn.  A whole CTA per row where there are few rows (a lone sequence has as many states as warps worked on it), a
-// few lanes where there are many.
-constexpr int kJoinThreads = 1024;
-
-template <int D, int kRowThreads>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs p, long long decode_warps) {
-    constexpr int kVecs = D / 4, kGroups = kRowThreads / kVecs, kRows = kJoinThreads / kRowThreads;
+// turn.  A lone sequence has as many states as warps worked on it (a hundred and more) and few rows: a CTA of 1024 threads
+// takes a row.  A large batch has thousands of rows of a few states: a group each.  In between 256 threads.  Bound by
+// latency: two rounds of dependent loads (where the states lie, the states).
+template <int D, int kRowThreads, int kThreads>
+__global__ void __launch_bounds__(kThreads) join_kernel(const DecodeArgs p, int decode_warps) {
+    constexpr int kVecs = D / 4, kGroups = kRowThreads / kVecs, kRows = kThreads / kRowThreads;
     __shared__ float4 s_acc[kRows][kGroups][kVecs];
     __shared__ float s_m[kRows][kGroups], s_l[kRows][kGroups];
     const int slot_row = threadIdx.x / kRowThreads, tid = threadIdx.x % kRowThreads;
     const int g = tid / kVecs, j = tid % kVecs;
     const int num_q = p.c.num_kv_heads * p.group;
-    const long long out_row = static_cast<long long>(blockIdx.x) * kRows + slot_row;
-    pdl_enter();
-    const bool valid = out_row < static_cast<long long>(p.num_seqs) * num_q;
-    const int b = valid ? static_cast<int>(out_row / num_q) : 0;
-    const int qh = valid ? static_cast<int>(out_row - static_cast<long long>(b) * num_q) : 0;
+    const int rows = p.num_seqs * num_q;
+    const int out_row = min(static_cast<int>(blockIdx.x) * kRows + slot_row, rows - 1);      // (the last CTA repeats its last row)
+    const int b = out_row / num_q, qh = out_row - b * num_q;
     const int kvh = qh / p.group, hg = qh - kvh * p.group;
+    pdl_enter();
 
     float m = kMInit, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -500,42 +498,42 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs p, 
         acc.w = acc.w * f + a.w * fi;
         m = n;
     };
-    const int shared_keys = p.header[0];
+    const int shared_keys = p.header[0], own_tiles = p.header[1], first = p.header[kHeaderInts + b], after = p.header[kHeaderInts + b + 1];
     const int heads = p.c.num_kv_heads * p.head_chunks;
-    const int prefix_segs = p.prefix_chunks * p.c.num_kv_heads;
     const int prefix_tiles = shared_keys / kTile;
-    const long long prefix_total = static_cast<long long>(prefix_segs) * prefix_tiles;
-    const long long total = prefix_total + static_cast<long long>(p.header[1]) * heads;
+    const long long prefix_total = static_cast<long long>(p.prefix_chunks * p.c.num_kv_heads) * prefix_tiles;
+    const long long total = prefix_total + static_cast<long long>(own_tiles) * heads;
     const long long warps = warps_in_use(total, decode_warps);
-    auto warp_of = [&](long long t) { return ((t + 1) * warps - 1) / total; };
-    auto take_slots = [&](const float* base, long long first, long long last, int cols, int col) {
-        const long long size = state_floats(cols, D);
-#pragma unroll 4
-        for (long long i = first + g; i <= last; i += kGroups) {
-            const float* const s = base + i * size;
-            take(s[col], s[cols + col], *reinterpret_cast<const float4*>(s + acc_offset(cols) + col * D + 4 * j));
-        }
+    // the warp that worked on tile t of the line: the last w with floor(total w / warps) <= t
+    auto warp_of = [&](long long t) {
+        const unsigned long long n = static_cast<unsigned long long>(t + 1) * static_cast<unsigned long long>(warps) - 1;
+        return n >> 32 == 0 ? static_cast<long long>(static_cast<unsigned>(n) / static_cast<unsigned>(total)) : static_cast<long long>(n / static_cast<unsigned long long>(total));
     };
-    if (valid && total > 0) {
-        if (prefix_total > 0) {
-            const int row = b * p.group + hg;
-            const long long seg = static_cast<long long>(kvh) * p.prefix_chunks + row / kPrefixCols;
-            const long long t0 = seg * prefix_tiles;
-            take_slots(p.prefix_states, seg + warp_of(t0), seg + warp_of(t0 + prefix_tiles - 1), kPrefixCols, row % kPrefixCols);
-        }
-        const int n = p.header[kHeaderInts + b + 1] - p.header[kHeaderInts + b];
-        if (n > 0) {
-            const int head = kvh * p.head_chunks + hg / kOwnCols;
-            const long long seg = static_cast<long long>(b) * heads + head;
-            const long long t0 = prefix_total + static_cast<long long>(p.header[kHeaderInts + b]) * heads + static_cast<long long>(head) * n;
-            take_slots(p.own_states, seg + warp_of(t0), seg + warp_of(t0 + n - 1), p.own_cols, hg % kOwnCols);
-        }
+    auto take_slots = [&](const float* base, long long from, int count, int cols, int col) {
+        const long long size = state_floats(cols, D);
+        const float* s = base + (from + g) * size;
+#pragma unroll 4
+        for (int i = g; i < count; i += kGroups, s += kGroups * size)
+            take(s[col], s[cols + col], *reinterpret_cast<const float4*>(s + acc_offset(cols) + col * D + 4 * j));
+    };
+    if (prefix_total > 0) {
+        const int row = b * p.group + hg;
+        const long long seg = static_cast<long long>(kvh) * p.prefix_chunks + row / kPrefixCols;
+        const long long t0 = seg * prefix_tiles, w0 = warp_of(t0);
+        take_slots(p.prefix_states, seg + w0, static_cast<int>(warp_of(t0 + prefix_tiles - 1) - w0) + 1, kPrefixCols, row % kPrefixCols);
     }
-    if (valid && p.block_splits > 0 && shared_keys > 0) {      // the prefix as the tensor-memory kernel left it
-        const long long rows = static_cast<long long>(p.num_seqs) * num_q;
+    if (after > first) {
+        const int n = after - first, head = kvh * p.head_chunks + hg / kOwnCols;
+        const long long seg = static_cast<long long>(b) * heads + head;
+        const long long t0 = prefix_total + static_cast<long long>(first) * heads + static_cast<long long>(head) * n, w0 = warp_of(t0);
+        take_slots(p.own_states, seg + w0, static_cast<int>(warp_of(t0 + n - 1) - w0) + 1, p.own_cols, hg % kOwnCols);
+    }
+    if (p.block_splits > 0 && shared_keys > 0) {      // the prefix as the tensor-memory kernel left it
+#pragma unroll 4
         for (int i = g; i < p.block_splits; i += kGroups) {
-            const long long at = i * rows + out_row;
-            take(p.block_ml[2 * at], p.block_ml[2 * at + 1], *reinterpret_cast<const float4*>(p.block_acc + at * D + 4 * j));
+            const long long at = static_cast<long long>(i) * rows + out_row;
+            const float2 ml = *reinterpret_cast<const float2*>(p.block_ml + 2 * at);
+            take(ml.x, ml.y, *reinterpret_cast<const float4*>(p.block_acc + at * D + 4 * j));
         }
     }
     if constexpr (kGroups > 1) {
@@ -546,19 +544,29 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const DecodeArgs p, 
         }
         __syncthreads();
         if (g != 0) return;
-        m = kMInit;
+        float top = kMInit;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) top = fmaxf(top, s_m[slot_row][i]);
         l = 0.0f;
         acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int i = 0; i < kGroups; ++i) take(s_m[slot_row][i], s_l[slot_row][i], s_acc[slot_row][i][j]);
+#pragma unroll 8
+        for (int i = 0; i < kGroups; ++i) {
+            const float f = ex2f(s_m[slot_row][i] - top);
+            const float4 a = s_acc[slot_row][i][j];
+            l = fmaf(s_l[slot_row][i], f, l);
+            acc.x = fmaf(a.x, f, acc.x);
+            acc.y = fmaf(a.y, f, acc.y);
+            acc.z = fmaf(a.z, f, acc.z);
+            acc.w = fmaf(a.w, f, acc.w);
+        }
     }
-    if (!valid) return;
     uint2 w = make_uint2(0u, 0u);         // no key seen: zero
     if (l != 0.0f) {
         const float inv = 1.0f / l;
         w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
         w.y = pack_bf16x2(acc.z * inv, acc.w * inv);
     }
-    st_vec8(p.out + out_row * D + 4 * j, w);
+    st_vec8(p.out + static_cast<long long>(out_row) * D + 4 * j, w);
 }
 
 template <int D>
@@ -571,14 +579,18 @@ int launch_decode(const DecodeArgs& a, cudaStream_t stream, const char* fn) {
     return host::check_launch(fn);
 }
 
+template <int D, int kRowThreads, int kThreads>
+void launch_join_as(const DecodeArgs& a, int rows, cudaStream_t stream) {
+    constexpr int kRows = kThreads / kRowThreads;
+    host::launch<join_kernel<D, kRowThreads, kThreads>>(dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(kThreads), 0, stream, a,
+                                                        decode_ctas() * kDecWarps);
+}
 template <int D>
 int launch_join(const DecodeArgs& a, cudaStream_t stream, const char* fn) {
-    const long long rows = static_cast<long long>(a.num_seqs) * a.c.num_kv_heads * a.group;
-    const long long warps = static_cast<long long>(decode_ctas()) * kDecWarps;
-    if (rows <= 4 * host::num_sms())
-        host::launch<join_kernel<D, kJoinThreads>>(dim3(static_cast<unsigned>(rows)), dim3(kJoinThreads), 0, stream, a, warps);
-    else
-        host::launch<join_kernel<D, D / 4>>(dim3(static_cast<unsigned>((rows + kJoinThreads / (D / 4) - 1) / (kJoinThreads / (D / 4)))), dim3(kJoinThreads), 0, stream, a, warps);
+    const int rows = a.num_seqs * a.c.num_kv_heads * a.group;
+    if (rows <= host::num_sms()) launch_join_as<D, 1024, 1024>(a, rows, stream);
+    else if (rows <= 8 * host::num_sms()) launch_join_as<D, 256, 256>(a, rows, stream);
+    else launch_join_as<D, D / 4, 256>(a, rows, stream);
     return host::check_launch(fn);
 }
 
