@@ -20,7 +20,7 @@
 // What is different from there, and why.
 // (1) K codes are operands as they lie in the cache: q is split into two E4M3 parts, q = hi + lo, and S = hi K^T + lo K^T.
 //     bf16 has 8 significant bits, E4M3 4: with the row scaled so that its largest |q| is in 128..256, every element
-//     above 2^-9 of it is exact, smaller ones are off by at most 2^-17 of it.  Two E4M3 products take the time of one f16
+//     above 2^-9 of it is exact, smaller ones are off by at most 2^-16 of it.  Two E4M3 products take the time of one f16
 //     product, and nothing has to convert K: clock stamps of the f16 form (0.80 ms on 8192 tokens, 32/8 heads of 128) had
 //     every product waiting for the converted K tile, and both row blocks in step behind it.
 // (2) The V scale is folded into the f16 V operand (one rounding of 2^-11, like a weight's) instead of riding in the
@@ -47,6 +47,7 @@ namespace paged {
 namespace {
 
 using namespace tc;
+using ws::group_or;
 
 // Bounded wait on an mbarrier phase that also ends when another thread of the CTA has given up (ws::wait_phase's contract):
 // the common case, a phase that is complete or completes within a few polls, is a loop of two instructions.
@@ -107,9 +108,14 @@ struct BlockArgs {
     int group;
     int heads_per_cta;
     int tokens_per_block;
+    int slot_mul;              // ceil(2^16 / tokens_per_block): exact for the 128 rows of a block
     int head_chunks;
     float scale_log2e;
 };
+
+// "W ready" exists once per W buffer: a warp may finish tile i + 1 (whose scores only wait for everyone to have READ those of
+// tile i) while another one still rescales O for tile i, and its arrival must not count for tile i.
+enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
 
 template <int D, int kBlocks>
 struct Geo {
@@ -130,10 +136,10 @@ struct Geo {
     static constexpr int kStageBytes = 2 * kRawBytes + 1024;
     static constexpr int kCstFloats = 3 * kKeys + 4;                        // K scales; where V scales ride in the exponent: log2, inverse; flags
     static constexpr int kSQ = 0;
-    static constexpr int kSK = kSQ + kBlocks * kQPart;
+    static constexpr int kSK = kSQ + kBlocks * 2 * kQPart;                  // (a block's 128 rows of hi, then of lo; at the end its rows of out)
     static constexpr int kSV = kSK + kStages * kStageBytes;
-    static constexpr int kSRow = kSV + kVBuffers * kTileBytes;                    // per block: maxima of |q| (two halves of a row), then the rows' factors
-    static constexpr int kSCst = kSRow + kBlocks * 2 * kRows * 4;           // [kCstRing]
+    static constexpr int kSRow = kSV + kVBuffers * kTileBytes;                    // per block: the rows' factors
+    static constexpr int kSCst = kSRow + kBlocks * kRows * 4;           // [kCstRing]
     static constexpr int kSPoison = kSCst + kCstRing * kCstFloats * 4;      // per V buffer and key: 0, or NaN
     static constexpr int kSBar = kSPoison + kVBuffers * kKeys * 4;
     static constexpr int kSmemBytes = kSBar + 512 + 1024;
@@ -146,11 +152,22 @@ struct Geo {
     static constexpr int kBarConv = kBarCst + kCstRing;
     static constexpr int kNumBars = kBarConv + 1;
     static_assert(8 * kNumBars + 4 * (4 + kStages) <= 512, "barrier area");
+    // arrivals per phase
+    __device__ static constexpr uint32_t bar_count(int i) {
+        if (i < kBarVReady) {
+            const int of = i % kBarsPerBlock;
+            // S: the product's completion, and the product warp for the rest that the tile needs; O: the completion; then the softmax warps
+            return of < kBarPV ? 2 : of < kBarSRead ? 1 : 8;
+        }
+        if (i < kBarVEmpty) return kConvThreads;
+        if (i < kBarFull) return kBlocks;
+        if (i < kBarEmpty) return 1 + 32;                       // the bulk copies' bytes, and the copy warp's lanes for their scales
+        if (i < kBarCst) return 1 + kConvThreads / 32;          // the S products, the conversion warps
+        if (i < kBarConv) return kKeys / 32;
+        return kConvThreads;
+    }
     static_assert(kSK % 1024 == 0 && kStageBytes % 1024 == 0 && kSV % 1024 == 0 && kTileBytes % 1024 == 0, "operand tiles are 1 KB aligned");
 };
-// "W ready" exists once per W buffer: a warp may finish tile i + 1 (whose scores only wait for everyone to have READ those of
-// tile i) while another one still rescales O for tile i, and its arrival must not count for tile i.
-enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
 enum TileFlag { kSlow = 16 };            // flags: bits 0..3 = sixteen-key groups that exist, 16 = V scales ride in the exponent
 
 // Shared-memory descriptor of an E4M3 operand with rows of D bytes (K-major): 128-byte swizzle for D = 128, 64-byte for 64.
@@ -212,15 +229,14 @@ __device__ __forceinline__ bool elect_one() {
 }
 // Whether a V scale is outside what the f16 operand holds.  (A NaN is not: it makes the operand NaN.)
 __device__ __forceinline__ bool outside_fold(float vs) { return vs != 0.0f && vs == vs && !(vs >= kFoldLow && vs <= kFoldHigh); }
-// two floats -> E4M3 codes hi and lo with x = hi + lo (lo: what hi leaves, rounded)
-__device__ __forceinline__ void split_e4m3x2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    hi = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-    uint32_t back, none;
-    e4m3x4_to_f16x2x2(hi, back, none);
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&back));
-    lo = __nv_cvt_float2_to_fp8x2(make_float2(x - b.x, y - b.y), __NV_SATFINITE, __NV_E4M3);
+// Two bf16 times a power of two -> E4M3 codes hi and lo: hi is the value cut after four significant bits, which E4M3 holds,
+// lo the four that are left.
+__device__ __forceinline__ void split_e4m3x2(uint32_t w, float down, uint32_t& hi, uint32_t& lo) {
+    const uint32_t top = w & 0xfff0fff0u;
+    const float2 x = mul2_rn(bf2_to_f2(w), splat2(down)), h = mul2_rn(bf2_to_f2(top), splat2(down));
+    hi = __nv_cvt_float2_to_fp8x2(h, __NV_SATFINITE, __NV_E4M3);
+    lo = __nv_cvt_float2_to_fp8x2(add2_rn(x, neg2(h)), __NV_SATFINITE, __NV_E4M3);
 }
-
 // The batch entry and the token tile of CTA `index` (of all token tiles of all entries); false: there is none.
 // Tiles are numbered from the one with the most keys down, so the long ones start first: depth = keys in units of a
 // tile's tokens, and for at most 32 entries the number of tiles beyond a depth is one warp sum.
@@ -301,44 +317,18 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     const int kvh = blockIdx.x / p.head_chunks;
     const int chunk = blockIdx.x - kvh * p.head_chunks;
 
-    if (tid == 0) {
-#pragma unroll
-        for (int g = 0; g < kBlocks; ++g) {
-            uint64_t* const bb = bars + g * G::kBarsPerBlock;
-            pipe::mbar_init(&bb[kBarQK], 2);              // the product's completion, and the product thread for the rest that the tile needs
-            pipe::mbar_init(&bb[kBarQK + 1], 2);
-            pipe::mbar_init(&bb[kBarPV], 1);
-            pipe::mbar_init(&bb[kBarPV + 1], 1);
-            pipe::mbar_init(&bb[kBarSRead], 8);
-            pipe::mbar_init(&bb[kBarWReady], 8);
-            pipe::mbar_init(&bb[kBarWReady + 1], 8);
+    if (warp == 1) {
+        for (int i = lane; i < G::kNumBars; i += 32) pipe::mbar_init(&bars[i], G::bar_count(i));
+        if (lane == 0) {
+            *gave_up = 0;
+            *least = INT_MAX;
         }
-#pragma unroll
-        for (int i = 0; i < kVBuffers; ++i) {
-            pipe::mbar_init(&bars[G::kBarVReady + i], G::kConvThreads);
-            pipe::mbar_init(&bars[G::kBarVEmpty + i], kBlocks);
-        }
-#pragma unroll
-        for (int i = 0; i < kStages; ++i) {
-            pipe::mbar_init(&bars[G::kBarFull + i], 1 + 32);                    // the bulk copies' bytes, and the copy warp's lanes for their scales
-            pipe::mbar_init(&bars[G::kBarEmpty + i], 1 + G::kConvThreads / 32);           // the S products, the conversion warps
-        }
-#pragma unroll
-        for (int i = 0; i < kCstRing; ++i) pipe::mbar_init(&bars[G::kBarCst + i], kKeys / 32);
-        pipe::mbar_init(&bars[G::kBarConv], G::kConvThreads);
-        *gave_up = 0;
-        *least = INT_MAX;
         pipe::mbar_init_fence();
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pipe::smem_u32(tmem_slot)), "r"(G::kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
     // ---- what this CTA works on.  The prefix kernel follows a kernel of the same call whose results it does not need, and
     //      which has seen its own predecessors complete before this one may start: it waits at its end instead. ----
     if constexpr (!kPrefix) pdl_wait();
@@ -375,6 +365,11 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             }
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
     const int all_tiles = (total_keys + kKeys - 1) / kKeys;
     const int j0 = static_cast<int>(static_cast<long long>(all_tiles) * blockIdx.z / gridDim.z);
     const int n_tiles = work ? static_cast<int>(static_cast<long long>(all_tiles) * (blockIdx.z + 1) / gridDim.z) - j0 : 0;
@@ -385,11 +380,11 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     uint64_t* const bb = bars + blk * G::kBarsPerBlock;
     const uint32_t tmem_s = tmem + blk * kTmemCols, tmem_o = tmem_s + kKeys, tmem_w = tmem_o + kD, tmem_q = tmem_w + kKeys / 2;
     // a block's 256 columns: S 64, O 128, W 32 (f16 pairs), lo part of Q 32 (four codes each)
-    const int q_off = G::kSQ + blk * G::kQPart;
+    const int q_off = G::kSQ + blk * 2 * G::kQPart;
 
     // a row of a block: its head slot and token (counted from token0); whether it exists; the last key it sees
     auto row_at = [&](int row, int& tok, int& head) {
-        const int slot = row / p.tokens_per_block;
+        const int slot = (row * p.slot_mul) >> 16;           // row / tokens_per_block
         tok = block_tok + (row - slot * p.tokens_per_block);
         const int hg = chunk * p.heads_per_cta + slot;
         head = kvh * p.group + hg;
@@ -413,56 +408,56 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
     const int seen_by_all = kPrefix ? *least : held;
 
     // ---- Q (softmax warps): bf16 -> two E4M3 parts, hi in shared memory, lo in tensor memory (products whose rows come from
-    //      there read a third of the shared memory: its port is what this kernel fills first).  A row is scaled by a power of two so that its
-    //      largest |q| lies in 2^7 .. 2^8; its scores take that back. ----
-    float* const row_amax = reinterpret_cast<float*>(sm + G::kSRow) + blk * 2 * kRows;
+    //      there read a third of the shared memory: its port is what this kernel fills first).  A row is scaled by a power of
+    //      two so that its largest |q| lies in 2^7 .. 2^8; its scores take that back.  D / 8 lanes read a row together; lo
+    //      goes through shared memory, because a tensor-memory store wants a row per thread. ----
+    float* const row_factor = reinterpret_cast<float*>(sm + G::kSRow) + blk * kRows;
     if (warp < G::kSoftmaxWarps && n_tiles > 0) {
-        constexpr int kHalf = D / 16;                        // 16-byte pieces of bf16 per thread: half a row
-        const int row = 32 * (wb & 3) + lane, part = wb >> 2;
-        int tok, head;
-        const bool valid = row_at(row, tok, head);
-        const uint4* const src = reinterpret_cast<const uint4*>(p.q + (valid ? (token0 + tok) * p.q_stride + static_cast<long long>(head) * D : 0)) + kHalf * part;
-        uint4 w[kHalf];
-        uint32_t amax2 = 0u;
+        constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes, kSteps = 16 / kRowsAtOnce;     // a warp takes 16 rows
+        const int sub = lane % kLanes, row0 = 16 * wb + lane / kLanes;
+        uint4 w[kSteps];
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) {
+        for (int i = 0; i < kSteps; ++i) {
+            int tok, head;
             w[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (valid) w[i] = src[i];
+            if (row_at(row0 + i * kRowsAtOnce, tok, head))
+                w[i] = *reinterpret_cast<const uint4*>(p.q + (token0 + tok) * p.q_stride + static_cast<long long>(head) * D + 8 * sub);
         }
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) amax2 = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax2, w[i].x), w[i].y), w[i].z), w[i].w);
-        const float lo_max = bf_lo(amax2), hi_max = bf_hi(amax2);
-        row_amax[part * kRows + row] = lo_max != lo_max ? lo_max : hi_max != hi_max ? hi_max : fmaxf(lo_max, hi_max);
-        named_sync(4 + blk, 256);
-        const float amax_a = row_amax[row], amax_b = row_amax[kRows + row];
-        const float amax = fmaxf(amax_a, amax_b);
-        named_sync(4 + blk, 256);                            // everyone has read the maxima
-        int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
-        e = amax > 0.0f ? max(-100, e) - 7 : 0;
-        float down = __int_as_float((127 - e) << 23);
-        // E4M3 conversion would saturate an infinite q: a row that holds one, or a NaN, gets NaN through its factor
-        const bool finite = amax_a <= 3.4e38f && amax_b <= 3.4e38f;
-        if (part == 0) row_amax[row] = finite ? fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23) : NAN;
-        if (p.scale_log2e < 0.0f) down = -down;
-        uint32_t lo_words[4 * (kHalf / 2)];
+        for (int i = 0; i < kSteps; ++i) {
+            const int row = row0 + i * kRowsAtOnce;
+            uint32_t top = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(abs_bf16x2(w[i].x), w[i].y), w[i].z), w[i].w);
 #pragma unroll
-        for (int i = 0; i < kHalf / 2; ++i) {                // sixteen values: one 16-byte piece of each part
-            const uint32_t words[8] = {w[2 * i].x, w[2 * i].y, w[2 * i].z, w[2 * i].w, w[2 * i + 1].x, w[2 * i + 1].y, w[2 * i + 1].z, w[2 * i + 1].w};
-            uint32_t hi[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint32_t h0, l0, h1, l1;
-                split_e4m3x2(bf_lo(words[2 * k]) * down, bf_hi(words[2 * k]) * down, h0, l0);
-                split_e4m3x2(bf_lo(words[2 * k + 1]) * down, bf_hi(words[2 * k + 1]) * down, h1, l1);
-                hi[k] = (h0 & 0xffffu) | (h1 << 16);
-                lo_words[4 * i + k] = (l0 & 0xffffu) | (l1 << 16);
-            }
-            const int at = q_off + code_at<D>(row, (kHalf / 2) * part + i);
-            *reinterpret_cast<uint4*>(sm + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            for (int o = kLanes / 2; o > 0; o >>= 1) top = max_nan_bf16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float lo_max = bf_lo(top), hi_max = bf_hi(top), amax = fmaxf(lo_max, hi_max);
+            int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
+            e = amax > 0.0f ? max(-100, e) - 7 : 0;
+            float down = __int_as_float((127 - e) << 23);
+            // E4M3 conversion would saturate an infinite q: a row that holds one, or a NaN, gets NaN through its factor
+            const bool finite = lo_max <= 3.4e38f && hi_max <= 3.4e38f;
+            if (sub == 0) row_factor[row] = finite ? fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23) : NAN;
+            if (p.scale_log2e < 0.0f) down = -down;
+            uint32_t h0, l0, h1, l1, h2, l2, h3, l3;
+            split_e4m3x2(w[i].x, down, h0, l0);
+            split_e4m3x2(w[i].y, down, h1, l1);
+            split_e4m3x2(w[i].z, down, h2, l2);
+            split_e4m3x2(w[i].w, down, h3, l3);
+            unsigned char* const at = sm + q_off + code_at<D>(row, sub >> 1) + 8 * (sub & 1);
+            *reinterpret_cast<uint2*>(at) = make_uint2((h0 & 0xffffu) | (h1 << 16), (h2 & 0xffffu) | (h3 << 16));
+            *reinterpret_cast<uint2*>(at + G::kQPart) = make_uint2((l0 & 0xffffu) | (l1 << 16), (l2 & 0xffffu) | (l3 << 16));
         }
-        tmem_st_words<4 * (kHalf / 2)>(tmem_q + (static_cast<uint32_t>(32 * (wb & 3)) << 16) + part * (4 * (kHalf / 2)), lo_words);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         fence_async_smem();
+        named_sync(4 + blk, 256);
+        constexpr int kPieces = D / 32;                      // 16-byte pieces of half a row
+        const int row = 32 * (wb & 3) + lane, part = wb >> 2;
+        uint32_t lo[4 * kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(sm + q_off + G::kQPart + code_at<D>(row, kPieces * part + i));
+            lo[4 * i] = v.x; lo[4 * i + 1] = v.y; lo[4 * i + 2] = v.z; lo[4 * i + 3] = v.w;
+        }
+        tmem_st_words<4 * kPieces>(tmem_q + (static_cast<uint32_t>(32 * (wb & 3)) << 16) + part * (4 * kPieces), lo);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     if (warp < G::kConvWarp0) named_sync(3, 32 * G::kConvWarp0);
@@ -476,7 +471,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
         int tok_a, tok_b, head_a, head_b;
         const bool valid_a = row_at(row_a, tok_a, head_a), valid_b = row_at(row_b, tok_b, head_b);
         const int qpos_a = valid_a ? last_key(tok_a) : INT_MAX, qpos_b = valid_b ? last_key(tok_b) : INT_MAX;
-        const float c_a = n_tiles > 0 ? row_amax[row_a] : 0.0f, c_b = n_tiles > 0 ? row_amax[row_b] : 0.0f;
+        const float c_a = n_tiles > 0 ? row_factor[row_a] : 0.0f, c_b = n_tiles > 0 ? row_factor[row_b] : 0.0f;
         float m_a = kMInit, m_b = kMInit, l_a = 0.0f, l_b = 0.0f;
         const float* const cst0 = reinterpret_cast<const float*>(sm + G::kSCst);
         // One tile.  The plain form (kAny false) is for tiles that every row sees whole and whose V
@@ -631,38 +626,58 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
             l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
             l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
             l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
-            const long long at_a = valid_a ? static_cast<long long>(token0 + tok_a) * p.num_q_heads + head_a : 0;
-            const long long at_b = valid_b ? static_cast<long long>(token0 + tok_b) * p.num_q_heads + head_b : 0;
             const bool states = p.state_ml != nullptr;
             const float unfold = 1.0f / static_cast<float>(1 << kFoldShift);
-            const float f_a = states ? unfold : (l_a == 0.0f ? 0.0f : unfold / l_a), f_b = states ? unfold : (l_b == 0.0f ? 0.0f : unfold / l_b);
+            const float f_a = states ? unfold : unfold / l_a, f_b = states ? unfold : unfold / l_b;
+            const bool none_a = l_a == 0.0f, none_b = l_b == 0.0f;     // a row that saw nothing is zero, whatever stale values met its zero weights
             const long long split = static_cast<long long>(blockIdx.z) * p.out_rows;
+            const long long at_a = split + (valid_a ? static_cast<long long>(token0 + tok_a) * p.num_q_heads + head_a : 0);
+            const long long at_b = split + (valid_b ? static_cast<long long>(token0 + tok_b) * p.num_q_heads + head_b : 0);
             if (states && c2 == 0) {
-                if (valid_a) *reinterpret_cast<float2*>(p.state_ml + 2 * (split + at_a)) = make_float2(m_a, l_a);
-                if (valid_b) *reinterpret_cast<float2*>(p.state_ml + 2 * (split + at_b)) = make_float2(m_b, l_b);
+                if (valid_a) *reinterpret_cast<float2*>(p.state_ml + 2 * at_a) = make_float2(m_a, l_a);
+                if (valid_b) *reinterpret_cast<float2*>(p.state_ml + 2 * at_b) = make_float2(m_b, l_b);
             }
+            // Finished rows go through shared memory (where the block's Q was) so that whole rows are stored: 16-byte pieces,
+            // their places swizzled by the row.
+            unsigned char* const row_a_at = sm + q_off + row_a * (2 * D);
+            unsigned char* const row_b_at = sm + q_off + row_b * (2 * D);
 #pragma unroll 1
-            for (int cb = 0; cb < D; cb += 32) {
-                uint32_t ov[16];
+            for (int cb = 0; cb < D; cb += 64) {
+                uint32_t ov[32];
                 if (n_tiles > 0) {
-                    tmem_ld_frag_x4(ov, tmem_o + my_lanes16 + cb);
+                    tmem_ld_frag_x8(ov, tmem_o + my_lanes16 + cb);
                 } else {
 #pragma unroll
-                    for (int g = 0; g < 16; ++g) ov[g] = 0u;
+                    for (int g = 0; g < 32; ++g) ov[g] = 0u;
                 }
-                // a row that saw nothing is zero, whatever stale values met its zero weights
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float2 va = l_a == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(__uint_as_float(ov[4 * g]) * f_a, __uint_as_float(ov[4 * g + 1]) * f_a);
-                    const float2 vb = l_b == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(__uint_as_float(ov[4 * g + 2]) * f_b, __uint_as_float(ov[4 * g + 3]) * f_b);
-                    const int d = cb + 8 * g + 2 * c2;
+                for (int g = 0; g < 8; ++g) {
+                    const float2 va = none_a ? make_float2(0.0f, 0.0f) : make_float2(__uint_as_float(ov[4 * g]) * f_a, __uint_as_float(ov[4 * g + 1]) * f_a);
+                    const float2 vb = none_b ? make_float2(0.0f, 0.0f) : make_float2(__uint_as_float(ov[4 * g + 2]) * f_b, __uint_as_float(ov[4 * g + 3]) * f_b);
                     if (states) {
-                        if (valid_a) *reinterpret_cast<float2*>(p.state_acc + (split + at_a) * D + d) = va;
-                        if (valid_b) *reinterpret_cast<float2*>(p.state_acc + (split + at_b) * D + d) = vb;
+                        const int d = cb + 8 * g + 2 * c2;
+                        if (valid_a) *reinterpret_cast<float2*>(p.state_acc + at_a * D + d) = va;
+                        if (valid_b) *reinterpret_cast<float2*>(p.state_acc + at_b * D + d) = vb;
                     } else {
-                        if (valid_a) *reinterpret_cast<uint32_t*>(p.out + at_a * D + d) = pack_bf16x2(va.x, va.y);
-                        if (valid_b) *reinterpret_cast<uint32_t*>(p.out + at_b * D + d) = pack_bf16x2(vb.x, vb.y);
+                        const int piece = cb / 8 + g;
+                        *reinterpret_cast<uint32_t*>(row_a_at + ((piece ^ (row_a & 7)) << 4) + 4 * c2) = pack_bf16x2(va.x, va.y);
+                        *reinterpret_cast<uint32_t*>(row_b_at + ((piece ^ (row_b & 7)) << 4) + 4 * c2) = pack_bf16x2(vb.x, vb.y);
                     }
+                }
+            }
+        }
+        if (p.state_ml == nullptr) {
+            const bool all = !group_or(4 + blk, 256, !ok);       // (whoever gave up comes here too)
+            if (all && work) {
+                constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
+                const int sub = lane % kLanes;
+#pragma unroll 4
+                for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+                    const int row = 16 * wb + i * kRowsAtOnce + lane / kLanes;
+                    int tok, head;
+                    if (row_at(row, tok, head))
+                        st_vec(p.out + (static_cast<long long>(token0 + tok) * p.num_q_heads + head) * D + 8 * sub,
+                               *reinterpret_cast<const uint4*>(sm + q_off + row * (2 * D) + ((sub ^ (row & 7)) << 4)));
                 }
             }
         }
@@ -687,7 +702,7 @@ __global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_ker
                     if (ok && i > 0) ok = wait_bar(&of[kBarSRead], (i - 1) & 1, gave_up, __LINE__, p.error_word);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t q_hi = q_tile + static_cast<uint64_t>(g * (G::kQPart >> 4));
+                    const uint64_t q_hi = q_tile + static_cast<uint64_t>(g * 2 * (G::kQPart >> 4));
                     const uint32_t d = tmem + g * kTmemCols, q_lo = d + kKeys + kD + kKeys / 2;
                     if (elect_one()) {
 #pragma unroll
@@ -924,6 +939,7 @@ void deal_heads(int group, BlockArgs& a) {
     a.head_chunks = (group + 3) / 4;
     a.heads_per_cta = (group + a.head_chunks - 1) / a.head_chunks;
     a.tokens_per_block = kRows / a.heads_per_cta;
+    a.slot_mul = (65536 + a.tokens_per_block - 1) / a.tokens_per_block;
 }
 
 // The K codes of a layer as rows of head_dim bytes, copied in boxes of one run of keys, swizzled as the products read them.
@@ -1074,7 +1090,7 @@ extern "C" int rh_flash_prefill_packed_bf16(void* out, const void* q, long long 
     RH_REQUIRE(q_stride >= static_cast<long long>(num_q_heads) * cache->head_dim, RH_ERR_INVALID_ARG, "%s: q_stride is below num_q_heads * head_dim", fn);
     RH_REQUIRE(host::aligned16(q) && q_stride % 8 == 0 && host::aligned16(partial_or_null), RH_ERR_MISALIGNED,
                "%s: q and partial must be 16-byte aligned, q_stride a multiple of 8", fn);
-    RH_REQUIRE((reinterpret_cast<uintptr_t>(out) & 7u) == 0, RH_ERR_MISALIGNED, "%s: out must be 8-byte aligned", fn);
+    RH_REQUIRE(host::aligned16(out), RH_ERR_MISALIGNED, "%s: out must be 16-byte aligned", fn);
     a.out = static_cast<__nv_bfloat16*>(out);
     a.q = static_cast<const __nv_bfloat16*>(q);
     a.rows = rows_or_null;

@@ -45,8 +45,8 @@ def _ptr(t: TensorOrPtr, dtype: Optional[torch.dtype] = None, numel: Optional[in
 
 
 def _stream(stream) -> Optional[int]:
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream or None
+    if stream is None:     # the current stream's handle without the Stream object around it: a launch is a few microseconds
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()) or None
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream or None
     return int(stream) or None
@@ -276,7 +276,7 @@ def _token_rows(t, num_tokens: int, heads: int, head_dim: int, name: str):
 
 
 def _on_device(cache, fn: str) -> None:
-    if cache.device_index != torch.cuda.current_device():
+    if cache.device_index != torch._C._cuda_getDevice():
         raise RhError(fn, 1, f"the cache is on device {cache.device_index}, the current device is {torch.cuda.current_device()}")
 
 

@@ -65,7 +65,7 @@ def decode(c, q, num_q, scale, shared=None, rows=None, layer=0, out=None, partia
     return out
 
 
-BLOCKS = dict(extra=2.0 * 2.0 ** -11, small_step=2.0 ** -25, q_step=2.0 ** -17)     # the tcgen05 form of the prefix rounds the V operand (code x f16 of the scale) to f16
+BLOCKS = dict(extra=2.0 * 2.0 ** -11, small_step=2.0 ** -25, q_step=2.0 ** -16)     # the tcgen05 form of the prefix rounds the V operand (code x f16 of the scale) to f16
 
 
 def check(c, out, q, scale, lens, rows=None, layer=0, what="", **hold):
