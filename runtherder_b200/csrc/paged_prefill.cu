@@ -125,6 +125,10 @@ struct Geo {
     static constexpr int kConvThreads = 128;
     static constexpr int kCopyWarp = kConvWarp0 + kConvThreads / 32;
     static constexpr int kThreads = 32 * (kCopyWarp + 1);
+    // One row block of a shared prefix is held to 96 registers a thread (as for a block of 640), so that its 480 threads leave
+    // a CTA of the decode kernel, which works on the sequences' own keys at the same time, room on the SM: 32 sequences
+    // with 32768 shared keys and one of their own 60.6 -> 51.0 us, 12 with 8192 and 600 31.2 -> 30.3 us.
+    static constexpr int kBoundThreads = kBlocks == 1 ? 640 : kThreads;
     static constexpr int kPieces = kKeys * (D / 16);                        // 16-byte pieces of a raw tile
     static constexpr int kPerConv = kPieces / kConvThreads;
     static constexpr int kTmem = kTmemCols * kBlocks;
@@ -293,7 +297,7 @@ __device__ __forceinline__ bool find_tile(const BlockArgs& p, int index, int til
 
 // grid (kv heads x head chunks, token tiles, key ranges)
 template <int D, int kBlocks, bool kPrefix>
-__global__ void __launch_bounds__(Geo<D, kBlocks>::kThreads, 1) paged_blocks_kernel(const BlockArgs p, const __grid_constant__ CUtensorMap k_map) {
+__global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo<D, kBlocks>::kThreads, 1) paged_blocks_kernel(const BlockArgs p, const __grid_constant__ CUtensorMap k_map) {
     using G = Geo<D, kBlocks>;
     extern __shared__ unsigned char raw_smem[];
     const uint32_t base = (pipe::smem_u32(raw_smem) + 1023u) & ~1023u;
