@@ -69,6 +69,43 @@ def test_bad_call_arguments():
     refused(INVALID, "rh_kv_pages_copy", c, A, A, 11, None)
 
 
+def decode(cache, out=A, q=A, stride=512, layer=0, rows=None, seqs=2, heads=4, partial=A, shared=None, length=None):
+    return ("rh_flash_decode_paged_bf16", out, q, stride, cache, layer, rows, seqs, heads, 0.1, partial, shared, length, None)
+
+
+def prefill(cache, out=A, q=A, stride=512, layer=0, rows=None, cu=A, tokens=4, seqs=2, heads=4, partial=A, splits=2):
+    return ("rh_flash_prefill_packed_bf16", out, q, stride, cache, layer, rows, cu, tokens, seqs, heads, 0.1, partial, splits, None)
+
+
+def test_bad_attention_arguments():
+    c = pages()
+    for call in (decode, prefill):
+        refused(INVALID, *call(None))
+        refused(DIM, *call(pages(head_dim=96)))
+        refused(INVALID, *call(pages(lens=None)))
+        for bad in (dict(out=None), dict(q=None), dict(partial=None), dict(layer=-1), dict(layer=2), dict(seqs=0), dict(seqs=5), dict(heads=0),
+                    dict(heads=3), dict(stride=511)):
+            refused(INVALID, *call(c, **bad))
+        for bad in (dict(q=A + 8), dict(stride=516), dict(partial=A + 8), dict(out=A + 2)):
+            refused(MISALIGNED, *call(c, **bad))
+        refused(DIM, *call(c, heads=1026, stride=1026 * 128))
+    refused(INVALID, *decode(c, shared=A))
+    refused(INVALID, *decode(c, length=A))
+    refused(INVALID, *decode(c, rows=A, seqs=4097))
+    refused(MISALIGNED, *decode(c, out=A + 4))
+    refused(MISALIGNED, *prefill(c, out=A + 8))
+    for bad in (dict(cu=None), dict(tokens=0), dict(splits=0), dict(splits=65)):
+        refused(INVALID, *prefill(c, **bad))
+
+
+def test_attention_scratch_sizes():
+    splits, floats = _lib.lib.rh_flash_prefill_packed_splits, _lib.lib.rh_flash_prefill_packed_scratch_floats
+    assert floats(100, 8, 128, 1) == 0 and floats(100, 8, 128, 0) == 0 and floats(0, 8, 128, 4) == 0
+    assert floats(100, 8, 128, 4) >= 4 * 100 * 8 * 130
+    assert floats(1 << 20, 64, 128, 16) > 1 << 32      # counted in 64 bits
+    assert splits(0, 1, 1, 8, 8, 128) == 1 and splits(4, 1, 100, 3, 2, 128) == 1
+
+
 def test_scratch_sizes():
     f = _lib.lib.rh_kv_pages_scratch_ints
     assert f(0, 1, 1) == 0 and f(1, 0, 1) == 0 and f(1, 1, 0) == 0
