@@ -34,6 +34,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -439,7 +440,8 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             float down = __int_as_float((127 - e) << 23);
             // E4M3 conversion would saturate an infinite q: a row that holds one, or a NaN, gets NaN through its factor
             const bool finite = lo_max <= 3.4e38f && hi_max <= 3.4e38f;
-            if (sub == 0) row_factor[row] = finite ? fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23) : NAN;
+            // (a normal number at least: a masked score times zero would be NaN, and whatever is that small changes no weight)
+            if (sub == 0) row_factor[row] = finite ? fmaxf(fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23), FLT_MIN) : NAN;
             if (p.scale_log2e < 0.0f) down = -down;
             uint32_t h0, l0, h1, l1, h2, l2, h3, l3;
             split_e4m3x2(w[i].x, down, h0, l0);
@@ -1035,7 +1037,7 @@ int launch_prefix(const DecodeArgs& d, int head_dim, cudaStream_t stream, const 
     a.out_rows = static_cast<long long>(d.num_seqs) * a.num_q_heads;
     a.num_tokens = d.num_seqs;
     a.num_seqs = d.num_seqs;
-    a.scale_log2e = d.scale_log2e == 0.0f ? 1.0e-30f : d.scale_log2e;
+    a.scale_log2e = d.scale_log2e;
     deal_heads(d.group, a);
     const int blocks = d.num_seqs > a.tokens_per_block ? 2 : 1;
     const unsigned tiles = static_cast<unsigned>((d.num_seqs + blocks * a.tokens_per_block - 1) / (blocks * a.tokens_per_block));
@@ -1105,7 +1107,7 @@ extern "C" int rh_flash_prefill_packed_bf16(void* out, const void* q, long long 
     a.out_rows = static_cast<long long>(num_tokens) * num_q_heads;
     a.num_tokens = num_tokens;
     a.num_seqs = num_seqs;
-    a.scale_log2e = scale == 0.0f ? 1.0e-30f : scale * paged::kLog2e;      // (a masked score times zero would be NaN)
+    a.scale_log2e = scale * paged::kLog2e;
     paged::deal_heads(num_q_heads / cache->num_kv_heads, a);
     if (num_splits > 1) {
         a.state_acc = partial_or_null;

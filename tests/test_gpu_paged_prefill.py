@@ -150,6 +150,14 @@ def test_softmax_scale_of_zero_and_below(scale):
     check(c, prefill(c, q, cu, 8, scale), q, [70, 5], [0, 40], scale)
 
 
+@pytest.mark.parametrize("scale,mul", [(0.0, 1e-25), (1e-30, 1e-20), (-1e-37, 1e-30), (1e-3, 1e-36)])
+def test_scores_that_vanish(scale, mul):
+    """Softmax scale times the queries' size below what fp32 holds: every visible key counts the same, masked ones not at all."""
+    c, q, cu = batch([70, 5], [0, 40], 8, 2, 128, 16, seed=12)
+    q = (q.float() * mul).to(torch.bfloat16)
+    check(c, prefill(c, q, cu, 8, scale), q, [70, 5], [0, 40], scale)
+
+
 def test_queries_of_widely_different_size_in_a_row():
     """Elements far below a row's largest one: what the two parts of q lose must stay within 2^-16 of it."""
     hq, hkv, dim = 8, 2, 128
