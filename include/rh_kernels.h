@@ -205,7 +205,8 @@ int rh_bias_rope_kv_fp8(void* q, void* k_out_or_null, const void* k_in, const vo
  * sequence, and everything that changes from step to step is device-resident, so a whole step can be recorded
  * into a CUDA graph.
  *
- * A call names its batch by `rows` (table row of every entry, each at most once; NULL: entry i is row i) and, for
+ * A call names its batch by `rows` (table row of every entry, each at most once: of entries that name the same row
+ * reserve, append and advance take the first and leave the others out; NULL: entry i is row i) and, for
  * packed tokens, by `cu_seqlens` (num_seqs + 1 non-decreasing offsets: tokens cu_seqlens[i] .. cu_seqlens[i+1]-1
  * belong to entry i; entries may be empty).  lens[row] is the number of tokens a row holds BEFORE the step, -1 for
  * an idle row; rh_kv_pages_advance adds the step's tokens at its end.  A step is: reserve; per layer append and
@@ -277,6 +278,7 @@ int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
  * num_splits > 1 (long histories in front of few new tokens) deals every row's keys to that many CTAs, whose states are
  * joined from partial_or_null: scratch of rh_flash_prefill_packed_scratch_floats(...) floats, 16-byte aligned, one per call that
  * may overlap in time.  rh_flash_prefill_packed_splits suggests a count (max_keys: the longest row with its new tokens).
+ * out, q and the scratch must be 16-byte aligned, q_stride a multiple of 8.  Several entries may name the same row here.
  * tcgen05 kernel, one CTA per SM holding 256 or all 512 of its tensor-memory columns for its lifetime. */
 int rh_flash_prefill_packed_splits(int num_tokens, int num_seqs, int max_keys, int num_q_heads, int num_kv_heads,
                                    int head_dim);
@@ -291,12 +293,12 @@ int rh_flash_prefill_packed_bf16(void* out, const void* q, long long q_stride, c
  * An entry whose row is idle, or that sees no key, gets zeros.  Several entries may name the same row here.
  *
  * shared_pages / shared_len (both or neither; device memory): the first *shared_len keys of every active entry lie in
- * the pages shared_pages[0], shared_pages[1], ... (e.g. the page-table row of any entry after rh_kv_pages_fork), and
+ * the pages shared_pages[0 .. pages_per_row - 1] (e.g. the page-table row of any entry after rh_kv_pages_fork), and
  * these are read once for all entries.  An entry that holds fewer keys attends those it holds.  The entries' own
  * table rows list the shared pages too; what is shared beyond a multiple of 256 keys is read through them.
  *
- * partial: caller-owned scratch of rh_flash_decode_paged_scratch_floats(...) floats, 16-byte aligned; calls that may
- * overlap in time need one each.  num_seqs <= 4096.  Two kernels, three where the prefix
+ * partial: caller-owned scratch of rh_flash_decode_paged_scratch_floats(...) floats, 16-byte aligned like q (out: 8-byte);
+ * calls that may overlap in time need one each.  num_seqs <= 4096, num_seqs * pages_per_row * page_size < 2^35.  Two kernels, three where the prefix
  * meets 17 or more query rows per kv head (it then runs on tcgen05); results do not depend on timing. */
 size_t rh_flash_decode_paged_scratch_floats(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
 int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_stride, const rh_kv_pages* cache, int layer,

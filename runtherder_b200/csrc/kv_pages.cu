@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendA
     const int row = p.rows != nullptr ? p.rows[s] : s;
     if (row < 0 || row >= p.c.num_rows) return;
     const int held = p.c.lens[row];
-    if (held < 0) return;
+    if (held < 0 || named_before(p.rows, s, row)) return;
     const long long pos = static_cast<long long>(held) + (token - p.cu_seqlens[s]);
     const long long column = pos >> p.c.page_shift;
     if (pos < 0 || column >= p.c.pages_per_row) return;
@@ -287,10 +287,11 @@ __global__ void __launch_bounds__(256) release_kernel(const Tables t, const int*
 
 __global__ void __launch_bounds__(256) advance_kernel(const Tables t, const int* rows, const int* cu_seqlens, int n) {
     pdl_enter();
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    const int i = (blockIdx.x * blockDim.x + threadIdx.x) / 32;      // a warp per entry
     if (i >= n) return;
     const int r = rows != nullptr ? rows[i] : i;
-    if (r >= 0 && r < t.num_rows && t.lens[r] >= 0) t.lens[r] += max(0, cu_seqlens[i + 1] - cu_seqlens[i]);
+    if (named_before(rows, i, r)) return;
+    if (threadIdx.x % 32 == 0 && r >= 0 && r < t.num_rows && t.lens[r] >= 0) t.lens[r] += max(0, cu_seqlens[i + 1] - cu_seqlens[i]);
 }
 
 // children[i] becomes a second owner of parents[i]'s whole pages and of a page of its own for the keys behind them.
@@ -667,7 +668,7 @@ extern "C" int rh_kv_pages_advance(const rh_kv_pages* cache, const int* rows_or_
     if (const int e = host::check_pages(cache, fn)) return e;
     RH_REQUIRE(cu_seqlens != nullptr, RH_ERR_INVALID_ARG, "%s: null pointer", fn);
     RH_REQUIRE(num_seqs >= 1 && num_seqs <= cache->num_rows, RH_ERR_INVALID_ARG, "%s: num_seqs must be in 1..num_rows", fn);
-    host::launch<paged::advance_kernel>(dim3(static_cast<unsigned>((num_seqs + 255) / 256)), dim3(256), 0, static_cast<cudaStream_t>(stream),
+    host::launch<paged::advance_kernel>(dim3(static_cast<unsigned>((num_seqs + 7) / 8)), dim3(256), 0, static_cast<cudaStream_t>(stream),
                                         paged::tables_of(cache), rows_or_null, cu_seqlens, num_seqs);
     return host::check_launch(fn);
 }

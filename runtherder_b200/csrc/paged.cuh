@@ -56,6 +56,15 @@ __device__ __forceinline__ int warp_find_last(const int* first, int n, int t) {
     return lo;
 }
 
+// Whether an entry in front of entry s names the same row (rows == null: never), found by the whole warp.  Of entries that
+// name a row twice the first counts.
+__device__ __forceinline__ bool named_before(const int* rows, int s, int row) {
+    if (rows == nullptr) return false;
+    bool found = false;
+    for (int i = threadIdx.x & 31; i < s; i += 32) found |= rows[i] == row;
+    return __any_sync(0xffffffffu, found);
+}
+
 }  // namespace paged
 
 namespace host {

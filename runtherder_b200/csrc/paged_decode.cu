@@ -616,6 +616,8 @@ extern "C" int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_
                "%s: shared_pages and shared_len go together", fn);
     RH_REQUIRE(num_seqs >= 1 && num_seqs <= paged::kMaxSeqs, RH_ERR_INVALID_ARG, "%s: num_seqs must be in 1..%d", fn, paged::kMaxSeqs);
     RH_REQUIRE(rows_or_null != nullptr || num_seqs <= cache->num_rows, RH_ERR_INVALID_ARG, "%s: more sequences than table rows", fn);
+    RH_REQUIRE(static_cast<long long>(num_seqs) * cache->pages_per_row * (cache->page_size / paged::kTile) <= INT_MAX, RH_ERR_UNSUPPORTED_DIM,
+               "%s: num_seqs * pages_per_row * page_size must stay below 2^35", fn);
     RH_REQUIRE(num_q_heads >= 1 && num_q_heads % cache->num_kv_heads == 0, RH_ERR_INVALID_ARG, "%s: num_q_heads must be a multiple of num_kv_heads", fn);
     RH_REQUIRE(num_q_heads <= 1024, RH_ERR_UNSUPPORTED_DIM, "%s: at most 1024 query heads", fn);
     RH_REQUIRE(q_stride >= static_cast<long long>(num_q_heads) * cache->head_dim, RH_ERR_INVALID_ARG, "%s: q_stride is below num_q_heads * head_dim", fn);

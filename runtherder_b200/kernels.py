@@ -254,13 +254,20 @@ def bias_rope_kv_fp8(q, k_out, k_in, v_in, q_bias, k_bias, v_bias, positions, in
 
 # ---- a batch of sequences in a paged cache (runtherder_b200.kv_cache.PagedKVCache) -----------------
 
-def _token_rows(t, num_tokens: int, heads: int, head_dim: int, name: str):
+def _cptr(cache, t, dtype, numel: Optional[int], name: str):
+    """_ptr for an argument of a call on `cache`: it must lie on the cache's device."""
+    if t is not None and not isinstance(t, int) and t.get_device() != cache.device_index:
+        raise RhError(name, 1, f"{name} must be on cuda:{cache.device_index}, where the cache is, got {t.device}")
+    return _ptr(t, dtype, numel, name)
+
+
+def _token_rows(cache, t, num_tokens: int, heads: int, head_dim: int, name: str):
     """Address and token stride of [num_tokens, heads, head_dim] bf16 whose tokens may lie apart (a slice of a
     fused projection); within a token the values are contiguous."""
     if isinstance(t, int):
         return t, heads * head_dim
-    if not t.is_cuda:
-        raise RhError(name, 1, f"{name} must be a CUDA tensor")
+    if t.get_device() != cache.device_index:
+        raise RhError(name, 1, f"{name} must be on cuda:{cache.device_index}, where the cache is, got {t.device}")
     if t.dtype != _BF:
         raise RhError(name, 1, f"{name} must have dtype {_BF}, got {t.dtype}")
     width = heads * head_dim
@@ -289,38 +296,38 @@ def _paged_call(cache, fn: str, *args) -> None:
 def kv_append_paged_fp8(cache, layer: int, k, v, cu_seqlens, num_tokens: int, num_seqs: int, rows=None, stream=None) -> None:
     """Quantises the packed batch's new keys and values [num_tokens, Hkv, D] into its rows' pages, at positions lens[row]
     and on.  Tokens at or behind cu_seqlens[num_seqs] are padding."""
-    kp, ks = _token_rows(k, num_tokens, cache.num_kv_heads, cache.head_dim, "k")
-    vp, vs = _token_rows(v, num_tokens, cache.num_kv_heads, cache.head_dim, "v")
-    _paged_call(cache, "rh_kv_append_paged_fp8", layer, kp, vp, ks, vs, _ptr(rows, _I32, num_seqs, "rows"),
-                _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, _stream(stream))
+    kp, ks = _token_rows(cache, k, num_tokens, cache.num_kv_heads, cache.head_dim, "k")
+    vp, vs = _token_rows(cache, v, num_tokens, cache.num_kv_heads, cache.head_dim, "v")
+    _paged_call(cache, "rh_kv_append_paged_fp8", layer, kp, vp, ks, vs, _cptr(cache, rows, _I32, num_seqs, "rows"),
+                _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, _stream(stream))
 
 
 def kv_pages_reserve(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
     """Gives the batch's active rows the pages that their new tokens need: the lowest free ones, in the order of the batch."""
-    _paged_call(cache, "rh_kv_pages_reserve", _ptr(rows, _I32, num_seqs, "rows"), _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
+    _paged_call(cache, "rh_kv_pages_reserve", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
                 num_seqs, _stream(stream))
 
 
 def kv_pages_release(cache, num_rows: int, rows=None, new_len: int = -1, stream=None) -> None:
     """Drops the rows' pages; new_len 0 starts an empty sequence, -1 leaves the row idle."""
-    _paged_call(cache, "rh_kv_pages_release", _ptr(rows, _I32, num_rows, "rows"), num_rows, new_len, _stream(stream))
+    _paged_call(cache, "rh_kv_pages_release", _cptr(cache, rows, _I32, num_rows, "rows"), num_rows, new_len, _stream(stream))
 
 
 def kv_pages_advance(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
     """lens[row] += the batch's new tokens, at the end of a step."""
-    _paged_call(cache, "rh_kv_pages_advance", _ptr(rows, _I32, num_seqs, "rows"), _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
+    _paged_call(cache, "rh_kv_pages_advance", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
                 num_seqs, _stream(stream))
 
 
 def kv_pages_fork(cache, parents, children, count: int, stream=None) -> None:
     """Row children[i] becomes a copy of row parents[i]: whole pages are shared, the filled part of the last one is copied."""
-    _paged_call(cache, "rh_kv_pages_fork", _ptr(parents, _I32, count, "parents"), _ptr(children, _I32, count, "children"), count,
+    _paged_call(cache, "rh_kv_pages_fork", _cptr(cache, parents, _I32, count, "parents"), _cptr(cache, children, _I32, count, "children"), count,
                 _stream(stream))
 
 
 def kv_pages_copy(cache, src, dst, count: int, stream=None) -> None:
     """Page dst[i] := page src[i] in every layer; the tables are left alone."""
-    _paged_call(cache, "rh_kv_pages_copy", _ptr(src, _I32, count, "src"), _ptr(dst, _I32, count, "dst"), count, _stream(stream))
+    _paged_call(cache, "rh_kv_pages_copy", _cptr(cache, src, _I32, count, "src"), _cptr(cache, dst, _I32, count, "dst"), count, _stream(stream))
 
 
 def kv_pages_compact(cache, stream=None) -> None:
@@ -337,14 +344,14 @@ def flash_decode_paged_scratch_floats(num_seqs: int, num_q_heads: int, num_kv_he
 def flash_decode_paged_bf16(out, q, cache, layer: int, num_seqs: int, num_q_heads: int, scale: float, partial, shared_pages=None,
                             shared_len=None, rows=None, stream=None) -> None:
     """One new token per entry attends keys 0..lens[row] of its row.  shared_pages / shared_len: the first *shared_len keys of
-    every entry lie in these pages (a page-table row) and are read once for all of them."""
+    every entry lie in these pages (a page-table row: pages_per_row entries) and are read once for all of them."""
     fn, D = "rh_flash_decode_paged_bf16", cache.head_dim
     _on_device(cache, fn)
-    qp, qs = _token_rows(q, num_seqs, num_q_heads, D, "q")
+    qp, qs = _token_rows(cache, q, num_seqs, num_q_heads, D, "q")
     need = flash_decode_paged_scratch_floats(num_seqs, num_q_heads, cache.num_kv_heads, D)
-    call(fn, _ptr(out, _BF, num_seqs * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _ptr(rows, _I32, num_seqs, "rows"), num_seqs,
-         num_q_heads, float(scale), _ptr(partial, _F32, need, "partial"), _ptr(shared_pages, _I32, None, "shared_pages"),
-         _ptr(shared_len, _I32, 1, "shared_len"), _stream(stream))
+    call(fn, _cptr(cache, out, _BF, num_seqs * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _cptr(cache, rows, _I32, num_seqs, "rows"), num_seqs,
+         num_q_heads, float(scale), _cptr(cache, partial, _F32, need, "partial"), _cptr(cache, shared_pages, _I32, cache.pages_per_row, "shared_pages"),
+         _cptr(cache, shared_len, _I32, 1, "shared_len"), _stream(stream))
 
 
 def flash_prefill_packed_splits(num_tokens: int, num_seqs: int, max_keys: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
@@ -365,8 +372,8 @@ def flash_prefill_packed_bf16(out, q, cache, layer: int, cu_seqlens, num_tokens:
     """A packed batch's new tokens attend causally: token i of an entry sees keys 0..lens[row] + i of its row."""
     fn, D = "rh_flash_prefill_packed_bf16", cache.head_dim
     _on_device(cache, fn)
-    qp, qs = _token_rows(q, num_tokens, num_q_heads, D, "q")
+    qp, qs = _token_rows(cache, q, num_tokens, num_q_heads, D, "q")
     need = flash_prefill_packed_scratch_floats(num_tokens, num_q_heads, D, num_splits)
-    call(fn, _ptr(out, _BF, num_tokens * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _ptr(rows, _I32, num_seqs, "rows"),
-         _ptr(cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, num_q_heads, float(scale),
-         _ptr(partial, _F32, need, "partial") if num_splits > 1 else None, num_splits, _stream(stream))
+    call(fn, _cptr(cache, out, _BF, num_tokens * num_q_heads * D, "out"), qp, qs, cache.desc, layer, _cptr(cache, rows, _I32, num_seqs, "rows"),
+         _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, num_q_heads, float(scale),
+         _cptr(cache, partial, _F32, need, "partial") if num_splits > 1 else None, num_splits, _stream(stream))

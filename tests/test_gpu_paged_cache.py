@@ -177,6 +177,37 @@ def test_append_is_the_cache_writer_at_the_rows_places(heads, dim, ps, new, stri
     same(c, want)
 
 
+@pytest.mark.parametrize("n", [3, 70])
+def test_a_row_named_twice_counts_once(n):
+    """reserve, append and advance take the first of the entries that name a row; the others' tokens go nowhere."""
+    c, m = make(layers=1, pages=200, ps=16, rows=80, per=4, heads=2, dim=64)
+    c.start(80)
+    m.release(range(80), 0)
+    rows = list(range(n - 1))
+    rows.insert(n // 2 + 1, rows[0])                     # the second one lies in front of others' tokens
+    new = [3 + i % 20 for i in range(n)]
+    k = torch.randn(sum(new), 2, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(torch.bfloat16)
+    cu, on = offsets(new), ints(rows)
+    first = [(r, x) for i, (r, x) in enumerate(zip(rows, new)) if r not in rows[:i]]
+    codes, scales = reference_append(k, 2, 64)
+    for _ in range(2):
+        c.reserve(cu, n, on)
+        m.reserve(rows, new)
+        m.check(c)
+        c.append(0, k, k, cu, sum(new), n, on)
+        for i, r in enumerate(rows):
+            if r in rows[:i]:
+                continue
+            at = sum(new[:i])
+            pos = torch.arange(m.lens[r], m.lens[r] + new[i])
+            page = torch.tensor([m.table[r][x] for x in (pos // 16).tolist()])
+            for got, want in ((c.k, codes), (c.v, codes), (c.k_scale, scales), (c.v_scale, scales)):
+                assert torch.equal(got[0, page.cuda(), :, (pos % 16).cuda()], want[at: at + new[i]]), (i, r)
+        c.advance(cu, n, on)
+        m.advance([r for r, _ in first], [x for _, x in first])
+        m.check(c)
+
+
 def test_empty_and_full_batches_and_identity_rows():
     c, m = make(pages=30, rows=4, per=6, heads=1)
     c.start(4)

@@ -92,6 +92,7 @@ def test_bad_attention_arguments():
     refused(INVALID, *decode(c, shared=A))
     refused(INVALID, *decode(c, length=A))
     refused(INVALID, *decode(c, rows=A, seqs=4097))
+    refused(DIM, *decode(pages(page_size=256, num_pages=1 << 20, num_rows=1 << 8, pages_per_row=1 << 20), rows=A, seqs=256))
     refused(MISALIGNED, *decode(c, out=A + 4))
     refused(MISALIGNED, *prefill(c, out=A + 8))
     for bad in (dict(cu=None), dict(tokens=0), dict(splits=0), dict(splits=65)):
