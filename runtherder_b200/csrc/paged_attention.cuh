@@ -81,7 +81,8 @@ __device__ __forceinline__ long long warps_in_use(long long total, long long war
 
 inline int decode_ctas() { return 4 * host::num_sms(); }
 
-// Query rows per kv head (entries x group) from which the tensor-memory kernel takes the prefix.
+// Query rows per kv head (entries x group) from which the tensor-memory kernel takes the prefix.  Whole calls with 8192 shared and
+// 100 own keys, 32/8 heads, mma.sync / tcgen05: 16 rows 18.4 / 22.5 us, 24 rows 23.9 / 22.5, 40 rows 31.7 / 22.8, 64 rows 45 / 28.
 constexpr int kBlockRows = 17;
 int prefix_splits(int num_seqs, int num_kv_heads, int group);
 

@@ -12,10 +12,10 @@
 //   O[128 x D] += W V        f16 (kind::f16): W = 2^(S c ks - m) in tensor memory, V = code x V scale in shared memory
 //
 //   softmax warps (8 per block)   scores -> weights; two rows x sixteen keys per thread
-//   product warps                 one thread issues S = Q K^T (of both blocks in turn), one per block O += W V
+//   product warps                 one warp issues S = Q K^T (of both blocks in turn), one per block O += W V
 //   conversion warps (4)          raw E4M3 V tiles -> f16 operand tiles, scales folded in; a tile's constants for the softmax
 //   copy warp                     fetches K tiles (tensor-map copies, swizzled as the product wants them), V tiles (bulk
-//                                 copies) and scales page by page, up to four tiles ahead
+//                                 copies) and scales page by page into four stages
 //
 // What is different from there, and why.
 // (1) K codes are operands as they lie in the cache: q is split into two E4M3 parts, q = hi + lo, and S = hi K^T + lo K^T.
@@ -31,6 +31,16 @@
 // (4) Rows carry their own last visible key, pages may be missing, and places that no row may see may hold anything: the
 //     tiles that reach past some row's last key (and only those) replace NaN codes of V by zero and mark the key, so that
 //     exactly the rows that see it get NaN.
+//
+// Measured (B200, 32/8 heads of 128).  One prompt of 8192 tokens 615 us = 890 TFLOP/s at full clocks (flash_prefill_ws.cu on a contiguous
+// cache: 718 us); six ragged prompts of 8192 tokens together 238 us = 607 TFLOP/s; the 32768 shared keys of 128 sequences about 85 us.
+// A tile of 64 keys takes two row blocks 1.35 us and costs 1152 cycles of products (tensor pipe 30 - 39 % busy) and 1024 of
+// exponentials; issue slots are 53 % busy.  What bounds it is the chain of a tile through a softmax warp (scores from tensor memory,
+// maximum, exponentials, weights to tensor memory, the product that frees them).  Tried without gain: 128-key tiles (765 us), the next
+// tile's scores loaded early (650 us, spills), exponentials partly as polynomials or left out altogether (no change), the two
+// blocks' softmax phases made exclusive (607 - 660 us), two one-block CTAs per SM (737 us).  A CTA costs 10.4 us besides its tiles:
+// 5.2 to fetch and split q, 2.8 to store its rows, 1.3 to find its tokens; ragged prompts with seven CTAs per SM lose a third
+// of their time to that.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -1114,7 +1124,10 @@ extern "C" int rh_flash_prefill_packed_bf16(void* out, const void* q, long long 
         a.state_ml = partial_or_null + static_cast<size_t>(num_splits) * a.out_rows * cache->head_dim;
     }
     const long long heads = static_cast<long long>(cache->num_kv_heads) * a.head_chunks;
-    // two row blocks per CTA once one-block CTAs are more than the SMs: a tile is converted once for twice the rows
+    // Two row blocks per CTA once one-block CTAs are more than the SMs: a tile is converted once for twice the rows, one and a half
+    // times a block's time.  One / two blocks: 128 tokens 9.8 / 13.1 us, 511 16.4 / 20.4; 1000 31.7 / 29.7, six prompts of 2048
+    // together 53.8 / 40.6, 700 tokens behind 2000 keys 90.8 / 62.8.  (Just above the border a short prompt without history, whose second
+    // wave would have few keys, loses: 600 tokens 18.8 / 21.8.)
     const int blocks = heads * paged::most_tiles(num_tokens, num_seqs, a.tokens_per_block) * num_splits > host::num_sms() ? 2 : 1;
     const long long tiles = paged::most_tiles(num_tokens, num_seqs, blocks * a.tokens_per_block);
     RH_REQUIRE(tiles <= 65535, RH_ERR_UNSUPPORTED_DIM, "%s: too many token tiles in one call (%lld)", fn, tiles);
