@@ -124,6 +124,13 @@ struct BlockArgs {
     float scale_log2e;
 };
 
+// What a CTA works on: its tokens (indexes into q, and how many exist from the first on), the keys in front of them and the keys that
+// any of its rows sees, and where they lie.
+struct Job {
+    const int* pages;
+    int token0, tokens, held, total_keys, work;
+};
+
 // "W ready" exists once per W buffer: a warp may finish tile i + 1 (whose scores only wait for everyone to have READ those of
 // tile i) while another one still rescales O for tile i, and its arrival must not count for tile i.
 enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
@@ -166,7 +173,8 @@ struct Geo {
     static constexpr int kBarCst = kBarEmpty + kStages;
     static constexpr int kBarConv = kBarCst + kCstRing;
     static constexpr int kNumBars = kBarConv + 1;
-    static_assert(8 * kNumBars + 4 * (4 + kStages) <= 512, "barrier area");
+    static constexpr int kJobAt = 8 * kNumBars + 4 * (4 + kStages);         // what the CTA works on, from the warp that looks it up
+    static_assert(kJobAt % 8 == 0 && kJobAt + static_cast<int>(sizeof(Job)) <= 512, "barrier area");
     // arrivals per phase
     __device__ static constexpr uint32_t bar_count(int i) {
         if (i < kBarVReady) {
@@ -348,42 +356,44 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
     //      which has seen its own predecessors complete before this one may start: it waits at its end instead. ----
     if constexpr (!kPrefix) pdl_wait();
     pdl_trigger();
-    int token0, tokens;              // the CTA's tokens: indexes into q, and how many exist from there on
-    int held, total_keys;            // keys in front of the CTA's first token; keys that any of its rows sees
-    const int* pages = nullptr;
+    Job* const job = reinterpret_cast<Job*>(sm + G::kSBar + G::kJobAt);
     const int tile_tokens = kBlocks * p.tokens_per_block;
-    bool work = true;
-    if constexpr (kPrefix) {
-        const int room = p.c.pages_per_row << p.c.page_shift;
-        const int n = min(*p.shared_len, room);
-        total_keys = n < kSharedAlign ? 0 : n - n % kSharedAlign;
-        token0 = blockIdx.y * tile_tokens;
-        tokens = p.num_tokens - token0;
-        held = 0;
-        pages = p.shared_pages;
-    } else {
-        int seq = 0, tile = 0;
-        work = find_tile(p, blockIdx.y, tile_tokens, seq, tile);
-        token0 = tokens = held = total_keys = 0;
-        if (work) {
-            const int first = p.cu_seqlens[seq], n = min(p.cu_seqlens[seq + 1], p.num_tokens) - first;
-            const int row = p.rows != nullptr ? p.rows[seq] : seq;
-            token0 = first + tile * tile_tokens;
-            tokens = n - tile * tile_tokens;
-            work = first >= 0 && tokens > 0;
-            if (row >= 0 && row < p.c.num_rows && p.c.lens[row] >= 0) {
-                const long long room = static_cast<long long>(p.c.pages_per_row) << p.c.page_shift;
-                held = p.c.lens[row] + tile * tile_tokens;
-                const long long seen = static_cast<long long>(held) + min(tokens, tile_tokens);
-                total_keys = static_cast<int>(seen < room ? seen : room);
-                pages = p.c.page_table + static_cast<size_t>(row) * p.c.pages_per_row;
+    if (warp == 2) {                 // (one warp: 24 of them waiting for the same loads and warp sums took twice as long)
+        Job j = {};
+        if constexpr (kPrefix) {
+            const int room = p.c.pages_per_row << p.c.page_shift;
+            const int n = min(*p.shared_len, room);
+            j.total_keys = n < kSharedAlign ? 0 : n - n % kSharedAlign;
+            j.token0 = blockIdx.y * tile_tokens;
+            j.tokens = p.num_tokens - j.token0;
+            j.pages = p.shared_pages;
+            j.work = 1;
+        } else {
+            int seq = 0, tile = 0;
+            if (find_tile(p, blockIdx.y, tile_tokens, seq, tile)) {
+                const int first = p.cu_seqlens[seq], n = min(p.cu_seqlens[seq + 1], p.num_tokens) - first;
+                const int row = p.rows != nullptr ? p.rows[seq] : seq;
+                j.token0 = first + tile * tile_tokens;
+                j.tokens = n - tile * tile_tokens;
+                j.work = first >= 0 && j.tokens > 0;
+                if (row >= 0 && row < p.c.num_rows && p.c.lens[row] >= 0) {
+                    const long long room = static_cast<long long>(p.c.pages_per_row) << p.c.page_shift;
+                    j.held = p.c.lens[row] + tile * tile_tokens;
+                    const long long seen = static_cast<long long>(j.held) + min(j.tokens, tile_tokens);
+                    j.total_keys = static_cast<int>(seen < room ? seen : room);
+                    j.pages = p.c.page_table + static_cast<size_t>(row) * p.c.pages_per_row;
+                }
             }
         }
+        if (lane == 0) *job = j;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const int token0 = job->token0, tokens = job->tokens, held = job->held, total_keys = __shfl_sync(0xffffffffu, job->total_keys, 0);
+    const bool work = __shfl_sync(0xffffffffu, job->work, 0) != 0;
+    const int* const pages = job->pages;
 
     const int all_tiles = (total_keys + kKeys - 1) / kKeys;
     const int j0 = static_cast<int>(static_cast<long long>(all_tiles) * blockIdx.z / gridDim.z);
@@ -424,24 +434,29 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
 
     // ---- Q (softmax warps): bf16 -> two E4M3 parts, hi in shared memory, lo in tensor memory (products whose rows come from
     //      there read a third of the shared memory: its port is what this kernel fills first).  A row is scaled by a power of
-    //      two so that its largest |q| lies in 2^7 .. 2^8; its scores take that back.  D / 8 lanes read a row together; lo
+    //      two so that its largest |q| lies in 2^7 .. 2^8; its scores take that back.  D / 16 lanes read a row together; lo
     //      goes through shared memory, because a tensor-memory store wants a row per thread. ----
     float* const row_factor = reinterpret_cast<float*>(sm + G::kSRow) + blk * kRows;
     if (warp < G::kSoftmaxWarps && n_tiles > 0) {
-        constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes, kSteps = 16 / kRowsAtOnce;     // a warp takes 16 rows
-        const int sub = lane % kLanes, row0 = 16 * wb + lane / kLanes;
-        uint4 w[kSteps];
+        constexpr int kLanes = D / 16, kRowsAtOnce = 32 / kLanes, kSteps = 16 / kRowsAtOnce;     // a warp takes 16 rows
+        const int sub = lane % kLanes, row0 = 16 * wb + lane / kLanes;      // a lane takes 8 values of each half of its rows
+        uint4 w[kSteps][2];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             int tok, head;
-            w[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (row_at(row0 + i * kRowsAtOnce, tok, head))
-                w[i] = *reinterpret_cast<const uint4*>(p.q + (token0 + tok) * p.q_stride + static_cast<long long>(head) * D + 8 * sub);
+            w[i][0] = w[i][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (row_at(row0 + i * kRowsAtOnce, tok, head)) {
+                const uint4* const src = reinterpret_cast<const uint4*>(p.q + (token0 + tok) * p.q_stride + static_cast<long long>(head) * D) + sub;
+                w[i][0] = src[0];
+                w[i][1] = src[kLanes];
+            }
         }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const int row = row0 + i * kRowsAtOnce;
-            uint32_t top = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(abs_bf16x2(w[i].x), w[i].y), w[i].z), w[i].w);
+            uint32_t top = 0u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) top = amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(amax_acc_bf16x2(top, w[i][h].x), w[i][h].y), w[i][h].z), w[i][h].w);
 #pragma unroll
             for (int o = kLanes / 2; o > 0; o >>= 1) top = max_nan_bf16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
             const float lo_max = bf_lo(top), hi_max = bf_hi(top), amax = fmaxf(lo_max, hi_max);
@@ -453,14 +468,17 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             // (a normal number at least: a masked score times zero would be NaN, and whatever is that small changes no weight)
             if (sub == 0) row_factor[row] = finite ? fmaxf(fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23), FLT_MIN) : NAN;
             if (p.scale_log2e < 0.0f) down = -down;
-            uint32_t h0, l0, h1, l1, h2, l2, h3, l3;
-            split_e4m3x2(w[i].x, down, h0, l0);
-            split_e4m3x2(w[i].y, down, h1, l1);
-            split_e4m3x2(w[i].z, down, h2, l2);
-            split_e4m3x2(w[i].w, down, h3, l3);
-            unsigned char* const at = sm + q_off + code_at<D>(row, sub >> 1) + 8 * (sub & 1);
-            *reinterpret_cast<uint2*>(at) = make_uint2((h0 & 0xffffu) | (h1 << 16), (h2 & 0xffffu) | (h3 << 16));
-            *reinterpret_cast<uint2*>(at + G::kQPart) = make_uint2((l0 & 0xffffu) | (l1 << 16), (l2 & 0xffffu) | (l3 << 16));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t h0, l0, h1, l1, h2, l2, h3, l3;
+                split_e4m3x2(w[i][h].x, down, h0, l0);
+                split_e4m3x2(w[i][h].y, down, h1, l1);
+                split_e4m3x2(w[i][h].z, down, h2, l2);
+                split_e4m3x2(w[i][h].w, down, h3, l3);
+                unsigned char* const at = sm + q_off + code_at<D>(row, (sub + h * kLanes) >> 1) + 8 * (sub & 1);
+                *reinterpret_cast<uint2*>(at) = make_uint2((h0 & 0xffffu) | (h1 << 16), (h2 & 0xffffu) | (h3 << 16));
+                *reinterpret_cast<uint2*>(at + G::kQPart) = make_uint2((l0 & 0xffffu) | (l1 << 16), (l2 & 0xffffu) | (l3 << 16));
+            }
         }
         fence_async_smem();
         named_sync(4 + blk, 256);
