@@ -131,8 +131,9 @@ struct Job {
     int token0, tokens, held, total_keys, work;
 };
 
-// "W ready" exists once per W buffer: a warp may finish tile i + 1 (whose scores only wait for everyone to have READ those of
-// tile i) while another one still rescales O for tile i, and its arrival must not count for tile i.
+// Per block: S complete, O += W V complete and W ready, each for even and for odd tiles, and S read (where S has one buffer).
+// "W ready" is two because a warp may finish tile i + 1 (whose scores only wait for everyone to have READ those of tile i) while another
+// one still rescales O for tile i, and its arrival must not count for tile i.
 enum BlockBar { kBarQK = 0, kBarPV = 2, kBarSRead = 4, kBarWReady = 5 };
 
 template <int D, int kBlocks>
@@ -150,6 +151,14 @@ struct Geo {
     static constexpr int kPieces = kKeys * (D / 16);                        // 16-byte pieces of a raw tile
     static constexpr int kPerConv = kPieces / kConvThreads;
     static constexpr int kTmem = kTmemCols * kBlocks;
+    // A block's 256 columns.  D = 128: S 64, O 128, W (f16 pairs) 32, lo part of Q (four codes each) 32.  D = 64: S twice, O 64,
+    // W_i over the columns of S_i; no warp waits for the others to have read S, nor for the last product to have read W.  One prompt of
+    // 8192 tokens, heads of 64: 513 us as for 128, 480 - 490 so; 700 tokens behind 12000 keys 140 / 137.  Heads of 128 have the
+    // columns for it only with lo in shared memory, which their products fill first: six ragged prompts 228 / 233 us.
+    static constexpr bool kTwoS = D == 64;
+    static constexpr int kOCol = kTwoS ? 2 * kKeys : kKeys, kWCol = kTwoS ? 0 : kOCol + D, kQCol = kWCol + kKeys / 2;
+    static constexpr int kSStep = kTwoS ? kKeys : 0;                        // from S (and W) of an even tile to that of an odd one
+    static_assert((kTwoS ? kOCol + D : kQCol + D / 4) <= kTmemCols, "tensor memory of a block");
     static constexpr int kDimBlocks = D / 64;                               // of the V operand
     static constexpr int kQPart = kRows * D;                                // q hi (or lo) of a block: rows of D bytes
     static constexpr int kTileBytes = kDimBlocks * kKeys * 128;             // an f16 V operand tile
@@ -403,8 +412,7 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
     const int wb = warp & 7;
     const int block_tok = blk * p.tokens_per_block;          // first token of the block, counted from token0
     uint64_t* const bb = bars + blk * G::kBarsPerBlock;
-    const uint32_t tmem_s = tmem + blk * kTmemCols, tmem_o = tmem_s + kKeys, tmem_w = tmem_o + kD, tmem_q = tmem_w + kKeys / 2;
-    // a block's 256 columns: S 64, O 128, W 32 (f16 pairs), lo part of Q 32 (four codes each)
+    const uint32_t tmem_s = tmem + blk * kTmemCols, tmem_o = tmem_s + G::kOCol, tmem_w = tmem_s + G::kWCol, tmem_q = tmem_s + G::kQCol;
     const int q_off = G::kSQ + blk * 2 * G::kQPart;
 
     // a row of a block: its head slot and token (counted from token0); whether it exists; the last key it sees
@@ -432,7 +440,7 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
     }
     const int seen_by_all = kPrefix ? *least : held;
 
-    // ---- Q (softmax warps): bf16 -> two E4M3 parts, hi in shared memory, lo in tensor memory (products whose rows come from
+    // ---- Q (softmax warps): bf16 -> two E4M3 parts, hi in shared memory, lo (D = 128) in tensor memory (products whose rows come from
     //      there read a third of the shared memory: its port is what this kernel fills first).  A row is scaled by a power of
     //      two so that its largest |q| lies in 2^7 .. 2^8; its scores take that back.  D / 16 lanes read a row together; lo
     //      goes through shared memory, because a tensor-memory store wants a row per thread. ----
@@ -481,17 +489,19 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             }
         }
         fence_async_smem();
-        named_sync(4 + blk, 256);
-        constexpr int kPieces = D / 32;                      // 16-byte pieces of half a row
-        const int row = 32 * (wb & 3) + lane, part = wb >> 2;
-        uint32_t lo[4 * kPieces];
+        if constexpr (!G::kTwoS) {
+            named_sync(4 + blk, 256);
+            constexpr int kPieces = D / 32;                      // 16-byte pieces of half a row
+            const int row = 32 * (wb & 3) + lane, part = wb >> 2;
+            uint32_t lo[4 * kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(sm + q_off + G::kQPart + code_at<D>(row, kPieces * part + i));
-            lo[4 * i] = v.x; lo[4 * i + 1] = v.y; lo[4 * i + 2] = v.z; lo[4 * i + 3] = v.w;
+            for (int i = 0; i < kPieces; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(sm + q_off + G::kQPart + code_at<D>(row, kPieces * part + i));
+                lo[4 * i] = v.x; lo[4 * i + 1] = v.y; lo[4 * i + 2] = v.z; lo[4 * i + 3] = v.w;
+            }
+            tmem_st_words<4 * kPieces>(tmem_q + (static_cast<uint32_t>(32 * (wb & 3)) << 16) + part * (4 * kPieces), lo);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
-        tmem_st_words<4 * kPieces>(tmem_q + (static_cast<uint32_t>(32 * (wb & 3)) << 16) + part * (4 * kPieces), lo);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     if (warp < G::kConvWarp0) named_sync(3, 32 * G::kConvWarp0);
@@ -515,10 +525,12 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             const int key0 = (j0 + i) * kKeys;
             const bool slow = kAny && (flags & kSlow) != 0;
             uint32_t sr[32];
-            tmem_ld_frag_x8(sr, tmem_s + my_lanes16);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bb[kBarSRead]);        // S may be overwritten by the next product
+            tmem_ld_frag_x8(sr, tmem_s + (i & 1) * G::kSStep + my_lanes16);
+            if constexpr (!G::kTwoS) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) pipe::mbar_arrive(&bb[kBarSRead]);    // S may be overwritten by the next product
+            }
             // pair 2 g: row a, keys 8 g + 2 c2 + {0, 1}; pair 2 g + 1: the same keys of row b.  (The constants lie in the
             // order of the weights: four for g = 2 a, 2 a + 1 at 16 a + 4 c2.)
             float2 sv[16];
@@ -610,12 +622,12 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             }
             l_a += sum_a.x + sum_a.y;
             l_b += sum_b.x + sum_b.y;
-            // W and O are free once O += W_{i-1} V_{i-1} is complete, a tile's work ago.
-            if (i > 0) {
+            // W and O are free once O += W_{i-1} V_{i-1} is complete, a tile's work ago.  (Of two buffers of W this one is.)
+            if (i > 0 && (!G::kTwoS || moved)) {
                 if (!wait_bar(&bb[kBarPV + ((i - 1) & 1)], ((i - 1) >> 1) & 1, gave_up, __LINE__, p.error_word)) return false;
                 tc_fence_after();
             }
-            tmem_st_frag_x4(tmem_w + my_lanes16, wv);
+            tmem_st_frag_x4(tmem_w + (i & 1) * G::kSStep + my_lanes16, wv);
             if (moved && i > 0) {
                 const float2 ca = splat2(corr_a), cb2 = splat2(corr_b);
 #pragma unroll 1
@@ -733,16 +745,24 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
 #pragma unroll
                 for (int g = 0; g < kBlocks; ++g) {
                     uint64_t* const of = bars + g * G::kBarsPerBlock;
-                    if (ok && i > 0) ok = wait_bar(&of[kBarSRead], (i - 1) & 1, gave_up, __LINE__, p.error_word);
+                    // S_i goes where S_{i-1} was, once that is read; of two buffers where S_{i-2} and W_{i-2} were, once O += W_{i-2} V_{i-2} is complete
+                    if constexpr (G::kTwoS) {
+                        if (ok && i > 1) ok = wait_bar(&of[kBarPV + (i & 1)], ((i >> 1) - 1) & 1, gave_up, __LINE__, p.error_word);
+                    } else {
+                        if (ok && i > 0) ok = wait_bar(&of[kBarSRead], (i - 1) & 1, gave_up, __LINE__, p.error_word);
+                    }
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t q_hi = q_tile + static_cast<uint64_t>(g * 2 * (G::kQPart >> 4));
-                    const uint32_t d = tmem + g * kTmemCols, q_lo = d + kKeys + kD + kKeys / 2;
+                    const uint32_t d = tmem + g * kTmemCols + (i & 1) * G::kSStep, q_lo = tmem + g * kTmemCols + G::kQCol;
                     if (elect_one()) {
 #pragma unroll
                         for (int s = 0; s < D / 32; ++s) umma_f8(d, q_hi + 2 * s, kd + 2 * s, kIdescQK, s > 0);
 #pragma unroll
-                        for (int s = 0; s < D / 32; ++s) umma_f8_ts(d, q_lo + 8 * s, kd + 2 * s, kIdescQK, true);
+                        for (int s = 0; s < D / 32; ++s) {
+                            if constexpr (G::kTwoS) umma_f8(d, q_hi + (G::kQPart >> 4) + 2 * s, kd + 2 * s, kIdescQK, true);
+                            else umma_f8_ts(d, q_lo + 8 * s, kd + 2 * s, kIdescQK, true);
+                        }
                         umma_commit(&of[kBarQK + (i & 1)]);
                         if (g == kBlocks - 1) umma_commit(&bars[G::kBarEmpty + stage]);        // K_i is free once these products are done
                     }
@@ -766,7 +786,7 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
                 if (elect_one()) {
 #pragma unroll
                     for (int s = 0; s < kKeys / 16; ++s)
-                        umma_f16_ts(tmem_o, tmem_w + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
+                        umma_f16_ts(tmem_o, tmem_w + (i & 1) * G::kSStep + s * 8, vd + s * (2048 >> 4), kIdescPV, i > 0 || s > 0);
                     umma_commit(&bb[kBarPV + (i & 1)]);
                     umma_commit(&bars[G::kBarVEmpty + buf]);
                 }
