@@ -33,14 +33,15 @@
 //     exactly the rows that see it get NaN.
 //
 // Measured (B200, 32/8 heads of 128).  One prompt of 8192 tokens 615 us = 890 TFLOP/s at full clocks (flash_prefill_ws.cu on a contiguous
-// cache: 718 us); six ragged prompts of 8192 tokens together 238 us = 607 TFLOP/s; the 32768 shared keys of 128 sequences about 85 us.
-// A tile of 64 keys takes two row blocks 1.35 us and costs 1152 cycles of products (tensor pipe 30 - 39 % busy) and 1024 of
+// cache: 718 us); six ragged prompts of 8192 tokens together 228 us = 634 TFLOP/s; the 32768 shared keys of 128 sequences about 85 us.
+// A tile of 64 keys takes two row blocks 1.3 us and costs 1152 cycles of products (tensor pipe 30 - 39 % busy) and 1024 of
 // exponentials; issue slots are 53 % busy.  What bounds it is the chain of a tile through a softmax warp (scores from tensor memory,
 // maximum, exponentials, weights to tensor memory, the product that frees them).  Tried without gain: 128-key tiles (765 us), the next
 // tile's scores loaded early (650 us, spills), exponentials partly as polynomials or left out altogether (no change), the two
-// blocks' softmax phases made exclusive (607 - 660 us), two one-block CTAs per SM (737 us).  A CTA costs 10.4 us besides its tiles:
-// 5.2 to fetch and split q, 2.8 to store its rows, 1.3 to find its tokens; ragged prompts with seven CTAs per SM lose a third
-// of their time to that.
+// blocks' softmax phases made exclusive (607 - 660 us), two one-block CTAs per SM (737 us).  A CTA costs 9.2 us besides its tiles: 4.2 to
+// fetch and split q, 2.7 to store its rows, 1.0 to find its tokens; ragged prompts with seven CTAs per SM lose a third of their
+// time to that.  CTAs that fetch further work by cluster launch control, with its first tiles on the way, took ragged prompts to 217 - 223
+// us, but short ones from 13.4 to 14.4 and one long one with 16-key pages from 680 to 702: not kept.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
