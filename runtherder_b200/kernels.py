@@ -283,14 +283,16 @@ def _token_rows(cache, t, num_tokens: int, heads: int, head_dim: int, name: str)
 
 
 def _on_device(cache, fn: str) -> None:
+    if cache.device_index < 0:
+        raise RhError(fn, 1, "the cache is not on a CUDA device")
     if cache.device_index != torch._C._cuda_getDevice():
         raise RhError(fn, 1, f"the cache is on device {cache.device_index}, the current device is {torch.cuda.current_device()}")
 
 
-def _paged_call(cache, fn: str, *args) -> None:
+def _paged_call(cache, stream, fn: str, *args) -> None:
     """An entry point whose first argument is a paged cache, on the cache's device."""
     _on_device(cache, fn)
-    call(fn, cache.desc, *args)
+    call(fn, cache.desc, *args, _stream(stream))
 
 
 def kv_append_paged_fp8(cache, layer: int, k, v, cu_seqlens, num_tokens: int, num_seqs: int, rows=None, stream=None) -> None:
@@ -298,41 +300,40 @@ def kv_append_paged_fp8(cache, layer: int, k, v, cu_seqlens, num_tokens: int, nu
     and on.  Tokens at or behind cu_seqlens[num_seqs] are padding."""
     kp, ks = _token_rows(cache, k, num_tokens, cache.num_kv_heads, cache.head_dim, "k")
     vp, vs = _token_rows(cache, v, num_tokens, cache.num_kv_heads, cache.head_dim, "v")
-    _paged_call(cache, "rh_kv_append_paged_fp8", layer, kp, vp, ks, vs, _cptr(cache, rows, _I32, num_seqs, "rows"),
-                _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs, _stream(stream))
+    _paged_call(cache, stream, "rh_kv_append_paged_fp8", layer, kp, vp, ks, vs, _cptr(cache, rows, _I32, num_seqs, "rows"),
+                _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"), num_tokens, num_seqs)
 
 
 def kv_pages_reserve(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
     """Gives the batch's active rows the pages that their new tokens need: the lowest free ones, in the order of the batch."""
-    _paged_call(cache, "rh_kv_pages_reserve", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
-                num_seqs, _stream(stream))
+    _paged_call(cache, stream, "rh_kv_pages_reserve", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
+                num_seqs)
 
 
 def kv_pages_release(cache, num_rows: int, rows=None, new_len: int = -1, stream=None) -> None:
     """Drops the rows' pages; new_len 0 starts an empty sequence, -1 leaves the row idle."""
-    _paged_call(cache, "rh_kv_pages_release", _cptr(cache, rows, _I32, num_rows, "rows"), num_rows, new_len, _stream(stream))
+    _paged_call(cache, stream, "rh_kv_pages_release", _cptr(cache, rows, _I32, num_rows, "rows"), num_rows, new_len)
 
 
 def kv_pages_advance(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
     """lens[row] += the batch's new tokens, at the end of a step."""
-    _paged_call(cache, "rh_kv_pages_advance", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
-                num_seqs, _stream(stream))
+    _paged_call(cache, stream, "rh_kv_pages_advance", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
+                num_seqs)
 
 
 def kv_pages_fork(cache, parents, children, count: int, stream=None) -> None:
     """Row children[i] becomes a copy of row parents[i]: whole pages are shared, the filled part of the last one is copied."""
-    _paged_call(cache, "rh_kv_pages_fork", _cptr(cache, parents, _I32, count, "parents"), _cptr(cache, children, _I32, count, "children"), count,
-                _stream(stream))
+    _paged_call(cache, stream, "rh_kv_pages_fork", _cptr(cache, parents, _I32, count, "parents"), _cptr(cache, children, _I32, count, "children"), count)
 
 
 def kv_pages_copy(cache, src, dst, count: int, stream=None) -> None:
     """Page dst[i] := page src[i] in every layer; the tables are left alone."""
-    _paged_call(cache, "rh_kv_pages_copy", _cptr(cache, src, _I32, count, "src"), _cptr(cache, dst, _I32, count, "dst"), count, _stream(stream))
+    _paged_call(cache, stream, "rh_kv_pages_copy", _cptr(cache, src, _I32, count, "src"), _cptr(cache, dst, _I32, count, "dst"), count)
 
 
 def kv_pages_compact(cache, stream=None) -> None:
     """Packs the used pages to the front of the pool; the page table and the reference counts follow."""
-    _paged_call(cache, "rh_kv_pages_compact", _stream(stream))
+    _paged_call(cache, stream, "rh_kv_pages_compact")
 
 
 def flash_decode_paged_scratch_floats(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:

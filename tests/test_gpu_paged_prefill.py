@@ -183,6 +183,33 @@ def test_long_prompt_sampled_tokens_and_repeatability():
     check_attention(out[8100:], q[8100:], k, v, 4001, scale, "behind", **HOLD)
 
 
+def test_pages_beyond_32_bit_offsets():
+    """Append, copy and packed prefill on pages that start more than 2^32 bytes into a layer's codes, in the second layer."""
+    from runtherder_b200 import kernels as K
+    from runtherder_b200.kv_cache import PagedKVCache
+    heads, hq, ps, dim, n = 8, 32, 256, 128, 300
+    pages = (1 << 32) // (heads * ps * dim) + 40
+    c = PagedKVCache(2, pages, ps, heads, dim, 1, 2)
+    mine = [pages - 1, pages - 7]
+    c.page_table.copy_(ints([mine]))
+    c.lens.fill_(0)
+    for p in mine:
+        c.ref_counts[p] = 1
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(n, heads, dim, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    cu, q = offsets([n]), queries(n, hq, dim, 3)
+    c.append(1, k, v, cu, n, 1)
+    kk, vv = row_contents(c, 1, 0, n)
+    for got, x in ((kk, k), (vv, v)):           # half a step of E4M3 is 2^-4 of the value, and 2^-10 / 448 of the row's largest below its normal range
+        x = x.double().transpose(0, 1)
+        assert ((got - x).abs() <= 2.0 ** -4 * 1.001 * x.abs() + x.abs().amax(-1, keepdim=True) * 2.0 ** -10 / 448).all()
+    assert not c.k[0, mine[0]].any() and not c.k[1, 0].any()
+    check(c, prefill(c, q, cu, hq, 0.09, layer=1), q, [n], [0], 0.09, layer=1)
+    K.kv_pages_copy(c, ints(mine), ints([3, 1]), 2)
+    for slab in (c.k, c.v, c.k_scale, c.v_scale):
+        assert torch.equal(slab[:, 3], slab[:, mine[0]]) and torch.equal(slab[:, 1], slab[:, mine[1]])
+
+
 def test_captured_and_replayed_with_other_lengths():
     from runtherder_b200 import kernels as K
     K.init(0)

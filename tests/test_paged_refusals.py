@@ -139,3 +139,13 @@ def test_python_class_checks_its_tensors():
         d.update(bad)
         with pytest.raises(RhError):
             PagedKVCache(**d)
+
+
+def test_a_cache_in_host_memory_is_refused():
+    from runtherder_b200 import kernels as K
+    c = PagedKVCache.from_tensors(**slabs())
+    k, cu = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: c.start(1), lambda: c.compact(), lambda: c.append(0, k, k, cu, 4, 3), lambda: c.reserve(cu, 3), lambda: c.fork(cu, cu, 2),
+                 lambda: K.flash_prefill_packed_bf16(k, k, c, 0, cu, 4, 3, 2, 0.1), lambda: K.flash_decode_paged_bf16(k, k, c, 0, 3, 2, 0.1, k)):
+        with pytest.raises(RhError):
+            call()
