@@ -19,12 +19,13 @@
 // bytes per key and kv head.  Scales never touch the operands: the K scale multiplies the fp32 score, the V scale
 // rides in the exponent of the weight (its log2 is added to the score), the denominator takes it out again.  A tile's
 // K codes and V codes are one run of memory each in this cache's layout: one lane fetches them with two bulk copies into the
-// warp's own ring, two tiles ahead, the scales come by one asynchronous copy per lane; there is no barrier among warps.
+// warp's own ring, a tile ahead, the scales come by one asynchronous copy per lane; there is no barrier among warps.
 //
-// Measured (B200, 32/8 heads of 128): 8 x 32768 keys 72 us = 5.0 TB/s, 64 x 2000 keys 40 us = 3.7 TB/s, of 6.5 for a copy; a
-// lone sequence of 8196 keys (24/8 heads) 14 us.  The decode kernel alone on 64 x 2000 keys takes 34 us (DRAM 53 % busy, issue slots
-// 45 %): a warp's tile is a chain of some 2000 cycles (wait, products, exponentials, transposes, products), sixteen warps of 128
-// registers fill an SM, and the E4M3 conversions alone are 14 us at one per cycle and SM.  What a small call waits for is latency:
+// Measured (B200, 32/8 heads of 128): 8 x 32768 keys 68 us = 5.3 TB/s, 64 x 2000 keys 38.8 us = 3.8 TB/s, of 6.5 for a copy; a
+// lone sequence of 8196 keys (24/8 heads) 14 us.  The decode kernel alone on 64 x 2000 keys takes 34 us (DRAM 56 % busy, issue slots
+// 46 %, 385 instructions per tile): a warp's tile is a chain of some 2000 cycles (wait, products, exponentials, transposes, products),
+// sixteen warps of 128 registers fill an SM (twenty of 96 spill: 64 x 2000 keys 44.9 us), and the E4M3 conversions alone are 8 us at one per
+// cycle and SM.  What a small call waits for is latency:
 // some 3 us to find its tiles and look up pages, the chain, and 4 us for the joining kernel.
 #include <cuda_fp16.h>
 
@@ -50,7 +51,8 @@ constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kTile = 16;              // keys per tile
 static_assert(kPrefixCols == 8 && kOwnCols == 8, "a segment has the eight columns of a product");
-constexpr int kStages = 3;             // tiles in a warp's ring
+constexpr int kStages = 2;             // tiles in a warp's ring (with three, 8 x 32768 keys take 72.5 us instead of 68: sixteen warps per SM have enough on the way)
+static_assert((kStages & (kStages - 1)) == 0, "counters wrap");
 constexpr int kDecCtas = 4;            // CTAs per SM
 constexpr float kLag = 8.0f;           // how far (log2) the running maximum may lie below the true one
 constexpr float kShift = 7.0f;         // weights enter the second product as 2^7 * weight (at most 2^15): small ones stay normal in f16
@@ -96,7 +98,7 @@ struct Walk {
     const DecodeArgs& p;
     unsigned char* ring;
     uint64_t* full;
-    uint32_t& turn;           // tiles this warp has taken from its ring so far, modulo 2 kStages: stage and parity of the next
+    uint32_t& turn;           // tiles this warp has taken from its ring so far: stage and parity of the next
     int lane, r, c;
 
     float o[kMB][4];
@@ -130,8 +132,7 @@ struct Walk {
                 here = ahead;
                 ahead = places(i + 33);
             }
-            const uint32_t stage = put >= kStages ? put - kStages : put;
-            put = put + 1 == 2 * kStages ? 0 : put + 1;
+            const uint32_t stage = put++ % kStages;
             uint64_t* const bar = full + stage;
             unsigned char* const dst = ring + stage * R::kStageBytes;
             const bool there = at >= 0;
@@ -207,16 +208,16 @@ struct Walk {
         for (int i = 0; i < tiles; ++i) {
             __syncwarp();                              // the stage that is filled next has been read by every lane
             if (i + kStages - 1 < tiles) issue(i + kStages - 1);
-            const uint32_t stage = turn >= kStages ? turn - kStages : turn;
-            ok = warp_wait(full + stage, turn >= kStages ? 1 : 0, __LINE__, p.error_word);
+            const uint32_t stage = turn % kStages;
+            ok = warp_wait(full + stage, (turn / kStages) & 1, __LINE__, p.error_word);
             if (!ok) {                                 // gave up: let the copies on their way land (bounded again), then leave
                 for (int k = 1; k < kStages && i + k < tiles; ++k) {
-                    const uint32_t t = (turn + k) % (2 * kStages);
-                    (void)warp_wait(full + t % kStages, t >= kStages ? 1 : 0, __LINE__, p.error_word, 1 << 12);
+                    const uint32_t t = turn + k;
+                    (void)warp_wait(full + t % kStages, (t / kStages) & 1, __LINE__, p.error_word, 1 << 12);
                 }
                 break;
             }
-            turn = turn + 1 == 2 * kStages ? 0 : turn + 1;
+            ++turn;
             if ((live >> (i & 31)) & 1u) {
                 if (i < plain) fold<false>(ring + stage * R::kStageBytes, key0 + i * kTile, qb, factor, see);
                 else fold<true>(ring + stage * R::kStageBytes, key0 + i * kTile, qb, factor, see);
