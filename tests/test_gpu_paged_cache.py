@@ -98,6 +98,27 @@ def test_copy_pages(ps, heads, dim, layers, n):
     assert c.status.tolist() == [0, 1 if n > 2 else 0]
 
 
+@pytest.mark.parametrize("pages,used", [(20000, 4000), (8192, 8192), (8193, 1), (16385, 9000), (3, 0)])
+def test_compact_pools_of_many_pages(pages, used):
+    rows, per = 100, 100
+    c, m = make(layers=1, pages=pages, ps=16, rows=rows, per=per, heads=1, dim=64)
+    rng = random.Random(pages)
+    for i, p in enumerate(rng.sample(range(pages), used)):
+        m.table[i % rows][i // rows] = p
+        m.refs[p] = 1
+    for i in range(min(used, 50)):                        # a second row lists some of them
+        p = m.table[i % rows][i // rows]
+        m.table[(i + 1) % rows][per - 1] = p
+        m.refs[p] = 2
+    c.page_table.copy_(ints(m.table))
+    c.ref_counts.copy_(ints(m.refs))
+    want = bits(c)
+    c.compact()
+    apply_moves(want, [(s, d, 16) for s, d in m.compact()])
+    m.check(c)
+    same(c, want)
+
+
 def test_fork_of_a_long_row_and_many_children():
     """More children than a warp has lanes, page lists longer than a warp is wide, and parents that are children themselves."""
     c, m = make(pages=900, ps=16, rows=80, per=70, heads=2, dim=64, layers=2)
