@@ -278,7 +278,8 @@ int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
  * num_splits > 1 (long histories in front of few new tokens) deals every row's keys to that many CTAs, whose states are
  * joined from partial_or_null: scratch of rh_flash_prefill_packed_scratch_floats(...) floats, 16-byte aligned, one per call that
  * may overlap in time.  rh_flash_prefill_packed_splits suggests a count (max_keys: the longest row with its new tokens).
- * out, q and the scratch must be 16-byte aligned, q_stride a multiple of 8.  Several entries may name the same row here.
+ * out, q and the scratch must be 16-byte aligned, q_stride a multiple of 8.  Several entries may name the same row here.  out must
+ * not overlap q.
  * tcgen05 kernel, one CTA per SM holding 256 or all 512 of its tensor-memory columns for its lifetime. */
 int rh_flash_prefill_packed_splits(int num_tokens, int num_seqs, int max_keys, int num_q_heads, int num_kv_heads,
                                    int head_dim);
