@@ -30,20 +30,13 @@ struct AppendArgs {
     int items_per_token;      // warps that share a token's 2 * kv heads rows
 };
 
-// scale = amax / 448 and codes e4m3_satfinite(x * (448 / amax)) of one head row spread over kLanes lanes with eight
-// values each: quantize_kv_fp8's arithmetic (NaN does not count for the maximum).
-template <int kLanes>
-__device__ __forceinline__ uint2 quantise_row(const uint4& x, float& scale) {
+// The largest |x| of a lane's eight values, as a pair of halves (NaN does not count).
+__device__ __forceinline__ __nv_bfloat162 amax_pair(const uint4& x) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
 #pragma unroll
     for (int i = 1; i < 4; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
-    const uint32_t mw = *reinterpret_cast<const uint32_t*>(&m);
-    const float amax = group_max<kLanes>(fmaxf(fmaxf(bf_lo(mw), bf_hi(mw)), 0.0f));
-    scale = quant_scale<448>(amax);
-    float y[8];
-    unpack8(x, y);
-    return pack_e4m3x8(y, quant_inv_scale<448>(amax));
+    return m;
 }
 
 constexpr int kAppendWarps = 8;
@@ -88,15 +81,32 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendA
     const int page = p.c.page_table[static_cast<size_t>(row) * p.c.pages_per_row + column];
     if (page < 0 || page >= p.c.num_pages) return;
     const int slot = static_cast<int>(pos) & ((1 << p.c.page_shift) - 1);
+    // quantize_kv_fp8's arithmetic: scale = amax / 448, codes e4m3_satfinite(x * (448 / amax)).  Two rows share a word for the maximum, and
+    // each of four lanes divides for one row.
+    uint32_t top[kAppendRows / 2];
+#pragma unroll
+    for (int j = 0; j < kAppendRows / 2; ++j) {
+        const __nv_bfloat162 a = amax_pair(x[2 * j]), b = amax_pair(x[2 * j + 1]);
+        __nv_bfloat162 m = __hmax2(__lows2bfloat162(a, b), __highs2bfloat162(a, b));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) m = __hmax2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        top[j] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+    static_assert(kAppendRows == 4 && kLanes >= 4, "a lane per row");
+    const uint32_t word = sub & 2 ? top[1] : top[0];
+    const float amax = fmaxf(sub & 1 ? bf_hi(word) : bf_lo(word), 0.0f);
+    const float scale = quant_scale<448>(amax), inv = quant_inv_scale<448>(amax);
 #pragma unroll
     for (int i = 0; i < kAppendRows; ++i) {
         const int r = first + i * kGroups + group;
-        float scale;
-        const uint2 codes = quantise_row<kLanes>(x[i], scale);
+        const float by = __shfl_sync(0xffffffffu, inv, (lane & ~(kLanes - 1)) + i);
+        float y[8];
+        unpack8(x[i], y);
+        const uint2 codes = pack_e4m3x8(y, by);
         if (r < 2 * Hkv) {
             const size_t key = key_index(p.c, page, r < Hkv ? r : r - Hkv) + slot;
             st_vec8((r < Hkv ? p.c.k : p.c.v) + key * D + 8 * sub, codes);
-            if (sub == 0) (r < Hkv ? p.c.k_scale : p.c.v_scale)[key] = scale;
+            if (sub == i) (r < Hkv ? p.c.k_scale : p.c.v_scale)[key] = scale;
         }
     }
 }
