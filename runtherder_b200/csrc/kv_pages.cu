@@ -27,7 +27,6 @@ struct AppendArgs {
     long long v_stride;
     int num_tokens;
     int num_seqs;
-    int items_per_token;      // warps that share a token's 2 * kv heads rows
 };
 
 // The largest |x| of a lane's eight values, as a pair of halves (NaN does not count).
@@ -51,11 +50,11 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendA
     constexpr int kLanes = D / 8;                 // lanes per head row, 16 bytes each
     constexpr int kGroups = 32 / kLanes;          // head rows a warp holds side by side
     const int lane = threadIdx.x & 31, sub = lane % kLanes, group = lane / kLanes;
-    const long long item = static_cast<long long>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
+    const long long index = static_cast<long long>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
     pdl_enter();
-    if (item >= static_cast<long long>(p.num_tokens) * p.items_per_token) return;
-    const int token = static_cast<int>(item / p.items_per_token);
-    const int first = static_cast<int>(item - static_cast<long long>(token) * p.items_per_token) * (kAppendRows * kGroups);
+    if (index >= p.num_tokens) return;
+    const int token = static_cast<int>(index);
+    const int first = blockIdx.y * (kAppendRows * kGroups);
     const int Hkv = p.c.num_kv_heads;
 
     uint4 x[kAppendRows];
@@ -100,9 +99,12 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendA
     for (int i = 0; i < kAppendRows; ++i) {
         const int r = first + i * kGroups + group;
         const float by = __shfl_sync(0xffffffffu, inv, (lane & ~(kLanes - 1)) + i);
-        float y[8];
-        unpack8(x[i], y);
-        const uint2 codes = pack_e4m3x8(y, by);
+        const float2 by2 = splat2(by);
+        auto four = [&](uint32_t lo, uint32_t hi) {
+            return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(mul2_rn(bf2_to_f2(lo), by2), __NV_SATFINITE, __NV_E4M3)) |
+                   static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(mul2_rn(bf2_to_f2(hi), by2), __NV_SATFINITE, __NV_E4M3)) << 16;
+        };
+        const uint2 codes = make_uint2(four(x[i].x, x[i].y), four(x[i].z, x[i].w));
         if (r < 2 * Hkv) {
             const size_t key = key_index(p.c, page, r < Hkv ? r : r - Hkv) + slot;
             st_vec8((r < Hkv ? p.c.k : p.c.v) + key * D + 8 * sub, codes);
@@ -650,10 +652,8 @@ extern "C" int rh_kv_append_paged_fp8(const rh_kv_pages* cache, int layer, const
     a.num_tokens = num_tokens;
     a.num_seqs = num_seqs;
     const int rows_per_warp = paged::kAppendRows * 32 / (cache->head_dim / 8);
-    a.items_per_token = (2 * cache->num_kv_heads + rows_per_warp - 1) / rows_per_warp;
-    const long long items = static_cast<long long>(num_tokens) * a.items_per_token;
-    RH_REQUIRE(items <= static_cast<long long>(INT_MAX) * paged::kAppendWarps, RH_ERR_UNSUPPORTED_DIM, "%s: too many tokens", fn);
-    const dim3 grid(static_cast<unsigned>((items + paged::kAppendWarps - 1) / paged::kAppendWarps)), block(32 * paged::kAppendWarps);
+    const dim3 grid((static_cast<unsigned>(num_tokens) + paged::kAppendWarps - 1) / paged::kAppendWarps,
+                    static_cast<unsigned>((2 * cache->num_kv_heads + rows_per_warp - 1) / rows_per_warp)), block(32 * paged::kAppendWarps);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (cache->head_dim == 128) host::launch<paged::append_kernel<128>>(grid, block, 0, s, a);
     else host::launch<paged::append_kernel<64>>(grid, block, 0, s, a);
