@@ -38,15 +38,16 @@ __device__ __forceinline__ __nv_bfloat162 amax_pair(const uint4& x) {
     return m;
 }
 
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 4;
 constexpr int kAppendRows = 4;    // head rows per lane group and warp, all in flight at once
 
 // A warp takes kAppendRows * 32 / (D / 8) consecutive head rows of one token (its K heads, then its V heads): eight
 // rows = 4 KB of reads in flight per warp at D = 128 (the rows are requested before their place is looked up).  Bound by
-// HBM for packed prompts, by latency for a decode step: 8192 tokens of 8 heads x 128 13.7 us = 3.7 TB/s of reads and writes (7.8 us at a
-// copy's rate), 32 tokens 3.5 us (a launch, two dependent rounds of loads, a store).
+// HBM for packed prompts, by latency for a decode step: 8192 tokens of 8 heads x 128 11.6 us = 4.4 TB/s of reads and writes (7.8 us at a
+// copy's rate), 32 tokens 2.9 us (a launch, two dependent rounds of loads, a store).  Issue slots bound it next to HBM: two rows' maxima in a
+// word, one lane's division per row and no division of indexes took it from 13.7 us.
 template <int D>
-__global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendArgs p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, 12) append_kernel(const AppendArgs p) {
     constexpr int kLanes = D / 8;                 // lanes per head row, 16 bytes each
     constexpr int kGroups = 32 / kLanes;          // head rows a warp holds side by side
     const int lane = threadIdx.x & 31, sub = lane % kLanes, group = lane / kLanes;
@@ -474,12 +475,20 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs p) {
     const int chunks = (p.num_kv_heads * ps * vecs_per_key + kMoveChunk - 1) / kMoveChunk;
     const long long items = static_cast<long long>(n) * p.num_layers * 2 * chunks;
     for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-        const int chunk = static_cast<int>(item % chunks);
-        long long rest = item / chunks;
-        const int slab = static_cast<int>(rest & 1);
-        rest >>= 1;
-        const int layer = static_cast<int>(rest % p.num_layers);
-        const int m = static_cast<int>(rest / p.num_layers);
+        int chunk, slab, layer, m;
+        if (items <= INT_MAX) {                                    // (64-bit divisions are calls of some 70 instructions each)
+            const unsigned rest = static_cast<unsigned>(item) / static_cast<unsigned>(chunks), block = rest >> 1;
+            chunk = static_cast<int>(static_cast<unsigned>(item) - rest * static_cast<unsigned>(chunks));
+            slab = static_cast<int>(rest & 1u);
+            m = static_cast<int>(block / static_cast<unsigned>(p.num_layers));
+            layer = static_cast<int>(block - static_cast<unsigned>(m) * static_cast<unsigned>(p.num_layers));
+        } else {
+            const long long rest = item / chunks, block = rest >> 1;
+            chunk = static_cast<int>(item - rest * chunks);
+            slab = static_cast<int>(rest & 1);
+            m = static_cast<int>(block / p.num_layers);
+            layer = static_cast<int>(block - static_cast<long long>(m) * p.num_layers);
+        }
         int src, dst, fill = ps;
         if (p.count >= 0) {
             src = p.src[m];
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs p) {
             if (e < total) {
                 int off = e;
                 if (fill != ps) {
-                    const int head = e / per_head;
+                    const int head = static_cast<int>(static_cast<unsigned>(e) / static_cast<unsigned>(per_head));
                     off = head * ps * vecs_per_key + (e - head * per_head);
                 }
                 at[i] = static_cast<size_t>(off);
