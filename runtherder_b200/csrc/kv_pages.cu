@@ -42,7 +42,7 @@ constexpr int kAppendWarps = 4;
 constexpr int kAppendRows = 4;    // head rows per lane group and warp, all in flight at once
 
 // A warp takes kAppendRows * 32 / (D / 8) consecutive head rows of one token (its K heads, then its V heads): eight
-// rows = 4 KB of reads in flight per warp at D = 128 (the rows are requested before their place is looked up).  Bound by
+// rows = 2 KB of reads in flight per warp at D = 128 (the rows are requested before their place is looked up).  Bound by
 // HBM for packed prompts, by latency for a decode step: 8192 tokens of 8 heads x 128 11.6 us = 4.4 TB/s of reads and writes (7.8 us at a
 // copy's rate), 32 tokens 2.9 us (a launch, two dependent rounds of loads, a store).  Issue slots bound it next to HBM: two rows' maxima in a
 // word, one lane's division per row and no division of indexes took it from 13.7 us.
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(256) advance_kernel(const Tables t, const int*
 }
 
 // Bookkeeping is one CTA's work: its steps depend on one another and their data are a few kilobytes, so it is bound by the
-// latency of some ten rounds of loads and barriers (a fork of 8 children 9.8 us with its copies, 13 us for the bookkeeping
+// latency of some ten rounds of loads and barriers (a fork of 8 children 9.5 us with its copies, 13 us for the bookkeeping
 // of 64 children with 31 shared pages each).
 //
 // children[i] becomes a second owner of parents[i]'s whole pages and of a page of its own for the keys behind them.
@@ -465,8 +465,8 @@ constexpr int kMoveChunk = kMoveThreads * kMoveVecs;               // pieces per
 
 // Work items: (move, layer, K or V, 16 KB piece of the block).  Bound by HBM: every byte is read and written once; a
 // thread has four 16-byte loads in flight, eight CTAs share an SM.  A compaction's CTAs also rewrite the page table.
-// Measured: 64 children of a row with a filled part of a 64-key page, 28 layers x 8 heads x 128 (416 MB read and written), 73 us with the
-// fork kernel in front = 5.7 TB/s; 1500 pages compacted 59 us; 4 pages copied 3.1 us.
+// Measured: 64 children of a row with a filled part of a 64-key page, 28 layers x 8 heads x 128 (416 MB read and written), 74 us with the
+// fork kernel in front = 5.6 TB/s; 1500 pages compacted 59 us; 4 pages copied 3.1 us.
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs p) {
     pdl_enter();
     const int n = p.count >= 0 ? p.count : p.moves[0];
