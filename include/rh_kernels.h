@@ -223,8 +223,8 @@ typedef struct rh_kv_pages {
     int32_t* page_table; /* [num_rows][pages_per_row], -1: no page */
     int32_t* lens;       /* [num_rows] tokens held, -1: idle */
     int32_t* ref_counts; /* [num_pages] rows that list the page, 0: free */
-    int32_t* status;     /* [2], only ever added to: pages that could not be provided; entries refused (a row or page out
-                            of range, a row named twice) */
+    int32_t* status;     /* [2], only ever added to: pages that could not be provided, each time they are asked for; entries
+                            refused (a row or page out of range, a row named twice) */
     int32_t* scratch;    /* rh_kv_pages_scratch_ints(num_rows, num_pages, pages_per_row) ints */
     int num_layers;
     int num_pages;
@@ -245,14 +245,17 @@ int rh_kv_append_paged_fp8(const rh_kv_pages* cache, int layer, const void* k, c
                            int num_seqs, void* stream);
 
 /* Gives every active row of the batch the pages for its new tokens.  Free pages are handed out lowest first, in
- * the order of the batch; where they run out the places stay -1 and status[0] counts what is missing. */
+ * the order of the batch; where they run out the places stay -1 and status[0] counts what is missing, and so it does for
+ * places behind the end of a table row, for a page id outside the pool and for a partly filled page that is gone. */
 int rh_kv_pages_reserve(const rh_kv_pages* cache, const int* rows_or_null, const int* cu_seqlens, int num_seqs,
                         void* stream);
 
 /* Drops the pages of `num_rows` rows; their length becomes new_len: 0 (a new, empty sequence) or -1 (idle). */
 int rh_kv_pages_release(const rh_kv_pages* cache, const int* rows_or_null, int num_rows, int new_len, void* stream);
 
-/* lens[row] += the batch's new tokens, for active rows. */
+/* lens[row] += the batch's new tokens, for active rows, up to the row's first place without a page: tokens from there on
+ * were not stored.  A row that got fewer pages than it asked for stops at a page's border and goes on from there once a
+ * later step's reserve finds pages; lens tells the caller how many of its tokens a row took. */
 int rh_kv_pages_advance(const rh_kv_pages* cache, const int* rows_or_null, const int* cu_seqlens, int num_seqs,
                         void* stream);
 

@@ -222,7 +222,9 @@ __device__ void first_owner(int* owner, int num_rows, const int* rows, int n) {
     __syncthreads();
 }
 
-// Gives every named row the pages it lacks for cu_seqlens[i + 1] - cu_seqlens[i] more tokens.
+// Gives every named row the pages it lacks for cu_seqlens[i + 1] - cu_seqlens[i] more tokens.  advance stops a row at its first place
+// without a page, so what a row lacks starts on a page's border.  Places that stay unusable all the same are counted: a partly filled
+// page that is gone (a new one would pass its stale slots off as the row's tokens) and a page outside the pool.
 __global__ void __launch_bounds__(kMetaThreads) reserve_kernel(const Tables t, const int* rows, const int* cu_seqlens, int n) {
     __shared__ int warp_sums[kMetaWarps];
     const Scratch s = scratch_of(t.scratch, t.num_rows, t.num_pages);
@@ -242,8 +244,15 @@ __global__ void __launch_bounds__(kMetaThreads) reserve_kernel(const Tables t, c
             const long long need = (static_cast<long long>(held) + more + (1 << t.page_shift) - 1) >> t.page_shift;
             to = static_cast<int>(need < t.pages_per_row ? need : t.pages_per_row);
             if (need > t.pages_per_row && lane == 0) atomicAdd(&t.status[0], static_cast<int>(need - t.pages_per_row));
-            for (int j = from + lane; j < to; j += 32) lack += t.page_table[static_cast<size_t>(r) * t.pages_per_row + j] < 0;
+            int unusable = 0;
+            for (int j = (held >> t.page_shift) + lane; j < to; j += 32) {
+                const int page = t.page_table[static_cast<size_t>(r) * t.pages_per_row + j];
+                if (page < 0 && j >= from) ++lack;
+                else unusable += page < 0 || page >= t.num_pages;
+            }
             lack = __reduce_add_sync(0xffffffffu, lack);
+            unusable = __reduce_add_sync(0xffffffffu, unusable);
+            if (unusable > 0 && lane == 0) atomicAdd(&t.status[0], unusable);
         } else if (lane == 0 && (!in_range || s.owner[r] != i)) {
             atomicAdd(&t.status[1], 1);
         }
@@ -300,13 +309,32 @@ __global__ void __launch_bounds__(256) release_kernel(const Tables t, const int*
     if (threadIdx.x == 0) t.lens[r] = new_len;
 }
 
+// lens += the new tokens, up to the row's first place without a page: the tokens from there on were not stored, and the next reserve
+// asks for that place again.  (Counting them in would leave the place empty for good, and the row's later tokens of that page with it.)
 __global__ void __launch_bounds__(256) advance_kernel(const Tables t, const int* rows, const int* cu_seqlens, int n) {
     pdl_enter();
     const int i = (blockIdx.x * blockDim.x + threadIdx.x) / 32;      // a warp per entry
     if (i >= n) return;
     const int r = rows != nullptr ? rows[i] : i;
-    if (named_before(rows, i, r)) return;
-    if (threadIdx.x % 32 == 0 && r >= 0 && r < t.num_rows && t.lens[r] >= 0) t.lens[r] += max(0, cu_seqlens[i + 1] - cu_seqlens[i]);
+    if (named_before(rows, i, r) || r < 0 || r >= t.num_rows) return;
+    const int held = t.lens[r], more = cu_seqlens[i + 1] - cu_seqlens[i], lane = threadIdx.x & 31;
+    if (held < 0 || more <= 0) return;
+    const long long room = static_cast<long long>(t.pages_per_row) << t.page_shift, all = static_cast<long long>(held) + more;
+    int end = static_cast<int>(all < room ? all : room);
+    for (int base = held >> t.page_shift; static_cast<long long>(base) << t.page_shift < end; base += 32) {
+        const int j = base + lane;
+        bool missing = false;
+        if (static_cast<long long>(j) << t.page_shift < end) {
+            const int page = t.page_table[static_cast<size_t>(r) * t.pages_per_row + j];
+            missing = page < 0 || page >= t.num_pages;
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, missing);
+        if (m != 0u) {
+            end = (base + __ffs(m) - 1) << t.page_shift;
+            break;
+        }
+    }
+    if (lane == 0 && end > held) t.lens[r] = end;
 }
 
 // Bookkeeping is one CTA's work: its steps depend on one another and their data are a few kilobytes, so it is bound by the

@@ -316,7 +316,7 @@ def kv_pages_release(cache, num_rows: int, rows=None, new_len: int = -1, stream=
 
 
 def kv_pages_advance(cache, cu_seqlens, num_seqs: int, rows=None, stream=None) -> None:
-    """lens[row] += the batch's new tokens, at the end of a step."""
+    """lens[row] += the batch's new tokens, at the end of a step; a row stops at its first place without a page."""
     _paged_call(cache, stream, "rh_kv_pages_advance", _cptr(cache, rows, _I32, num_seqs, "rows"), _cptr(cache, cu_seqlens, _I32, num_seqs + 1, "cu_seqlens"),
                 num_seqs)
 
