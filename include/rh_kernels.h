@@ -276,7 +276,7 @@ int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
 
 /* Causal attention of a packed batch's new tokens: token i of an entry attends keys 0 .. lens[row] + i of its row
  * (its keys were appended before this call).  out [num_tokens][num_q_heads][head_dim] bf16; q the same with q_stride
- * elements between tokens.  Tokens of an idle or unknown row get zeros; tokens at or behind cu_seqlens[num_seqs] are
+ * elements between tokens.  Tokens of an idle or unknown row get zeros, whatever their q holds; tokens at or behind cu_seqlens[num_seqs] are
  * padding, and their rows of out are left as they were.
  * num_splits > 1 (long histories in front of few new tokens) deals every row's keys to that many CTAs, whose states are
  * joined from partial_or_null: scratch of rh_flash_prefill_packed_scratch_floats(...) floats, 16-byte aligned, one per call that
@@ -294,7 +294,7 @@ int rh_flash_prefill_packed_bf16(void* out, const void* q, long long q_stride, c
 /* Attention of one new token per batch entry: out[b,h,:] = softmax_j(scale * q[b,h] . K[j]) V[j] over the keys
  * j = 0 .. lens[row of b] of its row (as rh_flash_decode_split_bf16: the new token's key sits at lens[row], appended
  * before this call).  out [num_seqs][num_q_heads][head_dim] bf16; q the same with q_stride elements between entries.
- * An entry whose row is idle, or that sees no key, gets zeros.  Several entries may name the same row here.
+ * An entry whose row is idle, or that sees no key, gets zeros, whatever its q holds.  Several entries may name the same row here.
  *
  * shared_pages / shared_len (both or neither; device memory): the first *shared_len keys of every active entry lie in
  * the pages shared_pages[0 .. pages_per_row - 1] (e.g. the page-table row of any entry after rh_kv_pages_fork), and

@@ -472,10 +472,11 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             int e = ((__float_as_int(amax) >> 23) & 0xff) - 127;
             e = amax > 0.0f ? max(-100, e) - 7 : 0;
             float down = __int_as_float((127 - e) << 23);
-            // E4M3 conversion would saturate an infinite q: a row that holds one, or a NaN, gets NaN through its factor
+            // A row that holds an infinity or a NaN has NaN among its lo codes (an infinity less itself), hence in every score; its
+            // factor stays a number, so that keys it must not see, at -inf, remain weightless and a row that sees none stays empty.
             const bool finite = lo_max <= 3.4e38f && hi_max <= 3.4e38f;
             // (a normal number at least: a masked score times zero would be NaN, and whatever is that small changes no weight)
-            if (sub == 0) row_factor[row] = finite ? fmaxf(fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23), FLT_MIN) : NAN;
+            if (sub == 0) row_factor[row] = finite ? fmaxf(fabsf(p.scale_log2e) * __int_as_float((127 + e) << 23), FLT_MIN) : 1.0f;
             if (p.scale_log2e < 0.0f) down = -down;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
