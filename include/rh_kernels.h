@@ -391,6 +391,10 @@ int rh_selfcheck_bounded_wait(int polls, int* gave_up_host, int* error_host);
  * returns normally and the context stays usable.  Diagnostic: allocates, synchronises. */
 int rh_selfcheck_role_wait(int tries, int* result_host);
 
+/* How rh_flash_decode_paged_bf16 deals `tiles` key tiles to `warps` warps: the warp that takes tile `tile`, and that warp's first
+ * tile, by the arithmetic that the kernels use (HOST pointers; host arithmetic, touches no device). */
+int rh_selfcheck_decode_line(long long tiles, long long warps, long long tile, long long* warp_host, long long* first_host);
+
 /* ---- Tuning knobs (process-wide; for experiments, defaults are the tuned values) --------- */
 
 /* key: "rows_ctas_per_sm", "swiglu_ctas_per_sm", "rope_warps_per_cta", "embed_ctas_per_sm",

@@ -66,6 +66,7 @@ SIGNATURES = {
     "rh_device_error": [_p],
     "rh_selfcheck_bounded_wait": [_i, _p, _p],
     "rh_selfcheck_role_wait": [_i, _p],
+    "rh_selfcheck_decode_line": [_ll, _ll, _ll, _p, _p],
     "rh_selftest_static": [_p, _i, _p],
 }
 _RESTYPES = {"rh_status_string": C.c_char_p, "rh_last_error_string": C.c_char_p,

@@ -79,6 +79,15 @@ __host__ __device__ constexpr long long state_floats(int cols, int dim) { return
 // four; 8 x 300 keys 10.6, 12.3, 13.0; 1 x 8196 keys 14.0, 15.8, 14.2.)
 __device__ __forceinline__ long long warps_in_use(long long total, long long warps) { return total < 1 ? 1 : (total < warps ? total : warps); }
 
+// The line of `total` tiles dealt to `warps` warps: warp w takes tiles line_start(w) .. line_start(w + 1) - 1, so tile t is that of the last
+// w with floor(total w / warps) <= t.  The short division wants both sides in 32 bits: the tiles of a call may be more (4096 entries that
+// name one long row), with t still small.
+__host__ __device__ inline long long line_start(long long total, long long warps, long long w) { return total * w / warps; }
+__host__ __device__ inline long long line_warp(long long total, long long warps, long long t) {
+    const unsigned long long n = static_cast<unsigned long long>(t + 1) * static_cast<unsigned long long>(warps) - 1, by = static_cast<unsigned long long>(total);
+    return (n | by) >> 32 == 0 ? static_cast<long long>(static_cast<unsigned>(n) / static_cast<unsigned>(by)) : static_cast<long long>(n / by);
+}
+
 inline int decode_ctas() { return 4 * host::num_sms(); }
 
 // Query rows per kv head (entries x group) from which the tensor-memory kernel takes the prefix.  Whole calls with 8192 shared and

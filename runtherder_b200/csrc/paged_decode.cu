@@ -423,8 +423,8 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(const Dec
     }
     const long long w = static_cast<long long>(blockIdx.x) * kDecWarps + warp;
     if (w >= warps) return;
-    long long t = total * w / warps;
-    const long long end = total * (w + 1) / warps;
+    long long t = line_start(total, warps, w);
+    const long long end = line_start(total, warps, w + 1);
 
     unsigned char* const ring = smem + warp * R::kWarpBytes;
     uint64_t* const full = bars + warp * kStages;
@@ -513,11 +513,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const DecodeArgs p, int 
     const long long prefix_total = static_cast<long long>(p.prefix_chunks * p.c.num_kv_heads) * prefix_tiles;
     const long long total = prefix_total + static_cast<long long>(own_tiles) * heads;
     const long long warps = warps_in_use(total, decode_warps);
-    // the warp that worked on tile t of the line: the last w with floor(total w / warps) <= t
-    auto warp_of = [&](long long t) {
-        const unsigned long long n = static_cast<unsigned long long>(t + 1) * static_cast<unsigned long long>(warps) - 1;
-        return n >> 32 == 0 ? static_cast<long long>(static_cast<unsigned>(n) / static_cast<unsigned>(total)) : static_cast<long long>(n / static_cast<unsigned long long>(total));
-    };
+    auto warp_of = [&](long long t) { return line_warp(total, warps, t); };      // the warp that worked on tile t
     auto take_slots = [&](const float* base, long long from, int count, int cols, int col) {
         const long long size = state_floats(cols, D);
         const float* s = base + (from + g) * size;
@@ -661,4 +657,14 @@ extern "C" int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_
     if (a.block_splits > 0)
         if (const int e = paged::launch_prefix(a, cache->head_dim, s, fn)) return e;
     return cache->head_dim == 128 ? paged::launch_join<128>(a, s, fn) : paged::launch_join<64>(a, s, fn);
+}
+
+extern "C" int rh_selfcheck_decode_line(long long tiles, long long warps, long long tile, long long* warp_host, long long* first_host) {
+    const char* const fn = "rh_selfcheck_decode_line";
+    RH_REQUIRE(warp_host && first_host, RH_ERR_INVALID_ARG, "%s: null pointer", fn);
+    RH_REQUIRE(tiles >= 1 && tiles <= (1LL << 42) && warps >= 1 && warps <= (1 << 16) && tile >= 0 && tile < tiles, RH_ERR_INVALID_ARG,
+               "%s: tiles must be in 1..2^42, warps in 1..2^16, tile in 0..tiles - 1", fn);
+    *warp_host = paged::line_warp(tiles, warps, tile);
+    *first_host = paged::line_start(tiles, warps, *warp_host);
+    return RH_OK;
 }
