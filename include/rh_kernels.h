@@ -226,13 +226,13 @@ typedef struct rh_kv_pages {
     int32_t* status;     /* [2], only ever added to: pages that could not be provided, each time they are asked for; entries
                             refused (a row or page out of range, a row named twice) */
     int32_t* scratch;    /* rh_kv_pages_scratch_ints(num_rows, num_pages, pages_per_row) ints */
-    int num_layers;
-    int num_pages;
+    int num_layers;      /* at most 4096 */
+    int num_pages;       /* at most 2^24; num_pages * num_kv_heads * page_size below 2^31 */
     int page_size;       /* a power of two, 16..256 */
-    int num_kv_heads;
+    int num_kv_heads;    /* at most 1024 */
     int head_dim;        /* 64 or 128 */
-    int num_rows;
-    int pages_per_row;
+    int num_rows;        /* at most 2^24 */
+    int pages_per_row;   /* num_rows * pages_per_row and pages_per_row * page_size below 2^30 */
 } rh_kv_pages;
 
 size_t rh_kv_pages_scratch_ints(int num_rows, int num_pages, int pages_per_row);

@@ -629,8 +629,9 @@ int check_pages(const rh_kv_pages* c, const char* fn) {
     RH_REQUIRE(c->page_size >= paged::kMinPage && c->page_size <= paged::kMaxPage && (c->page_size & (c->page_size - 1)) == 0,
                RH_ERR_UNSUPPORTED_DIM, "%s: page_size must be a power of two in 16..256", fn);
     RH_REQUIRE(c->head_dim == 64 || c->head_dim == 128, RH_ERR_UNSUPPORTED_DIM, "%s: head_dim must be 64 or 128", fn);
-    RH_REQUIRE(c->num_pages <= (1 << 24) && c->num_kv_heads <= 1024 && c->num_layers <= 4096, RH_ERR_UNSUPPORTED_DIM,
-               "%s: at most 2^24 pages, 1024 kv heads and 4096 layers", fn);
+    // (rows: the scratch's list of moves, three ints each, and a thread index of 32 per row stay within 32 bits)
+    RH_REQUIRE(c->num_pages <= (1 << 24) && c->num_rows <= (1 << 24) && c->num_kv_heads <= 1024 && c->num_layers <= 4096, RH_ERR_UNSUPPORTED_DIM,
+               "%s: at most 2^24 pages, 2^24 rows, 1024 kv heads and 4096 layers", fn);
     RH_REQUIRE(static_cast<long long>(c->num_rows) * c->pages_per_row <= INT_MAX / 2 && static_cast<long long>(c->pages_per_row) * c->page_size <= INT_MAX / 2,
                RH_ERR_UNSUPPORTED_DIM, "%s: num_rows * pages_per_row and pages_per_row * page_size must stay below 2^30", fn);
     RH_REQUIRE(static_cast<long long>(c->num_pages) * c->num_kv_heads * c->page_size <= INT_MAX, RH_ERR_UNSUPPORTED_DIM,

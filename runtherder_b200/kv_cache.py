@@ -125,6 +125,8 @@ class PagedKVCache:
             raise RhError("PagedKVCache", 2, "page_size must be a power of two in 16..256")
         if D not in (64, 128):
             raise RhError("PagedKVCache", 2, "head_dim must be 64 or 128")
+        if rows > 1 << 24:
+            raise RhError("PagedKVCache", 2, "at most 2^24 rows")
         self.num_layers, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = L, N, H, ps, D
         self.num_rows, self.pages_per_row = rows, per_row
         self.device_index = k.device.index if k.is_cuda else -1
