@@ -207,8 +207,9 @@ int rh_bias_rope_kv_fp8(void* q, void* k_out_or_null, const void* k_in, const vo
  *
  * A call names its batch by `rows` (table row of every entry, each at most once: of entries that name the same row
  * reserve, append and advance take the first and leave the others out; NULL: entry i is row i) and, for
- * packed tokens, by `cu_seqlens` (num_seqs + 1 non-decreasing offsets: tokens cu_seqlens[i] .. cu_seqlens[i+1]-1
- * belong to entry i; entries may be empty).  lens[row] is the number of tokens a row holds BEFORE the step, -1 for
+ * packed tokens, by `cu_seqlens` (num_seqs + 1 non-decreasing offsets from 0 on: tokens cu_seqlens[i] .. cu_seqlens[i+1]-1
+ * belong to entry i; entries may be empty; append and prefill leave out tokens behind their num_tokens, reserve and advance count
+ * what the offsets say).  lens[row] is the number of tokens a row holds BEFORE the step, -1 for
  * an idle row; rh_kv_pages_advance adds the step's tokens at its end.  A step is: reserve; per layer append and
  * attention; advance.  Rows, lengths and pages are checked where they are used: a token of an idle or unknown row,
  * or one whose page is missing (-1) or no page of the pool, is not stored, and such a page's keys are not attended.

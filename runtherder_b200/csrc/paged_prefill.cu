@@ -270,6 +270,8 @@ __device__ __forceinline__ void split_e4m3x2(uint32_t w, float down, uint32_t& h
     hi = __nv_cvt_float2_to_fp8x2(h, __NV_SATFINITE, __NV_E4M3);
     lo = __nv_cvt_float2_to_fp8x2(add2_rn(x, neg2(h)), __NV_SATFINITE, __NV_E4M3);
 }
+// The tokens of an entry that the call has (offsets may name more: the grid has CTAs for the call's).
+__device__ __forceinline__ int entry_tokens(const BlockArgs& p, int s) { return max(0, min(p.cu_seqlens[s + 1], p.num_tokens) - p.cu_seqlens[s]); }
 // The batch entry and the token tile of CTA `index` (of all token tiles of all entries); false: there is none.
 // Tiles are numbered from the one with the most keys down, so the long ones start first: depth = keys in units of a
 // tile's tokens, and for at most 32 entries the number of tiles beyond a depth is one warp sum.
@@ -278,7 +280,7 @@ __device__ __forceinline__ bool find_tile(const BlockArgs& p, int index, int til
     if (p.num_seqs <= 32) {
         int n = 0, behind = 0;
         if (lane < p.num_seqs) {
-            n = (max(0, p.cu_seqlens[lane + 1] - p.cu_seqlens[lane]) + tile_tokens - 1) / tile_tokens;
+            n = (entry_tokens(p, lane) + tile_tokens - 1) / tile_tokens;
             const int row = p.rows != nullptr ? p.rows[lane] : lane;
             if (row >= 0 && row < p.c.num_rows) behind = max(0, p.c.lens[row]) / tile_tokens;
         }
@@ -304,7 +306,7 @@ __device__ __forceinline__ bool find_tile(const BlockArgs& p, int index, int til
     int before = 0;
     for (int base = 0; base < p.num_seqs; base += 32) {
         const int s = base + lane;
-        const int n = s < p.num_seqs ? (max(0, p.cu_seqlens[s + 1] - p.cu_seqlens[s]) + tile_tokens - 1) / tile_tokens : 0;
+        const int n = s < p.num_seqs ? (entry_tokens(p, s) + tile_tokens - 1) / tile_tokens : 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
         } else {
             int seq = 0, tile = 0;
             if (find_tile(p, blockIdx.y, tile_tokens, seq, tile)) {
-                const int first = p.cu_seqlens[seq], n = min(p.cu_seqlens[seq + 1], p.num_tokens) - first;
+                const int first = p.cu_seqlens[seq], n = entry_tokens(p, seq);
                 const int row = p.rows != nullptr ? p.rows[seq] : seq;
                 j.token0 = first + tile * tile_tokens;
                 j.tokens = n - tile * tile_tokens;
