@@ -26,8 +26,11 @@
 // (2) The V scale is folded into the f16 V operand (one rounding of 2^-11, like a weight's) instead of riding in the
 //     exponent: no per-key additions and multiplications in the softmax.  f16 holds vs * 448 only for vs in 2^-22 .. 2^-1
 //     (with a common factor of 2^8); a tile with a scale outside keeps the exponent form, and both add up in one O.
-// (3) The running maximum may lag the true one by up to 2^8: weights stay below 2^8, exact enough in f16, sums are fp32,
-//     and O is rescaled a handful of times per row instead of on most tiles.
+// (3) The running maximum may lag the true one by up to 2^8, so that O is rescaled a handful of times per row instead of on most
+//     tiles.  Weights carry a factor of 2^7: they stay below 2^15, and what f16 loses of small ones is below 2^-32 of the largest
+//     (unshifted it was 2^-25: over 8192 keys that may be 2^-12 of the output, over 128k keys 2^-8, all of it missing from the
+//     numerator and present in the denominator).  Each weight is rounded to f16 once, 2^-11; the denominator sums the unrounded
+//     fp32 weights.
 // (4) Rows carry their own last visible key, pages may be missing, and places that no row may see may hold anything: the
 //     tiles that reach past some row's last key (and only those) replace NaN codes of V by zero and mark the key, so that
 //     exactly the rows that see it get NaN.
@@ -100,6 +103,7 @@ constexpr int kFoldShift = 8;            // V operand = code * vs * 2^8
 constexpr float kFoldLow = 2.384185791015625e-07f;    // 2^-22
 constexpr float kFoldHigh = 0.5f;
 constexpr float kLag = 8.0f;             // how far (log2) the running maximum may lie below the true one
+constexpr float kShift = 7.0f;           // weights are 2^7 * weight, at most 2^15: f16 holds them down to 2^-31 of the row's largest
 
 struct BlockArgs {
     Layer c;
@@ -604,7 +608,7 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
                 l_a *= corr_a;
                 l_b *= corr_b;
             }
-            const unsigned long long f2_a = both(f_a), f2_b = both(f_b), neg_a = both(-m_a), neg_b = both(-m_b);
+            const unsigned long long f2_a = both(f_a), f2_b = both(f_b), neg_a = both(kShift - m_a), neg_b = both(kShift - m_b);
             float2 sum_a = make_float2(0.0f, 0.0f), sum_b = make_float2(0.0f, 0.0f);
             // word 4 (g / 2) + g % 2: row a, keys 8 g + 2 c2 + {0, 1}; + 2: row b.  In tensor memory that is pair 8 (g / 2) +
             // 2 c2 + g % 2 of the row, so V's rows are laid out in that order.
@@ -684,8 +688,8 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
             const long long at_a = split + (valid_a ? static_cast<long long>(token0 + tok_a) * p.num_q_heads + head_a : 0);
             const long long at_b = split + (valid_b ? static_cast<long long>(token0 + tok_b) * p.num_q_heads + head_b : 0);
             if (states && c2 == 0) {
-                if (valid_a) *reinterpret_cast<float2*>(p.state_ml + 2 * at_a) = make_float2(m_a, l_a);
-                if (valid_b) *reinterpret_cast<float2*>(p.state_ml + 2 * at_b) = make_float2(m_b, l_b);
+                if (valid_a) *reinterpret_cast<float2*>(p.state_ml + 2 * at_a) = make_float2(m_a - kShift, l_a);
+                if (valid_b) *reinterpret_cast<float2*>(p.state_ml + 2 * at_b) = make_float2(m_b - kShift, l_b);
             }
             // Finished rows go through shared memory (where the block's Q was) so that whole rows are stored: 16-byte pieces,
             // their places swizzled by the row.
