@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(kMetaThreads) reserve_kernel(const Tables t, c
         const int held = in_range ? t.lens[r] : -1;
         int from = 0, to = 0, lack = 0;
         if (in_range && s.owner[r] == i && held >= 0 && more > 0) {
-            from = (held + (1 << t.page_shift) - 1) >> t.page_shift;
+            const long long first = (static_cast<long long>(held) + (1 << t.page_shift) - 1) >> t.page_shift;
+            from = static_cast<int>(first < t.pages_per_row ? first : t.pages_per_row);      // (a length may be anything)
             const long long need = (static_cast<long long>(held) + more + (1 << t.page_shift) - 1) >> t.page_shift;
             to = static_cast<int>(need < t.pages_per_row ? need : t.pages_per_row);
             if (need > t.pages_per_row && lane == 0) atomicAdd(&t.status[0], static_cast<int>(need - t.pages_per_row));

@@ -276,6 +276,8 @@ __device__ __forceinline__ void split_e4m3x2(uint32_t w, float down, uint32_t& h
 }
 // The tokens of an entry that the call has (offsets may name more: the grid has CTAs for the call's).
 __device__ __forceinline__ int entry_tokens(const BlockArgs& p, int s) { return max(0, min(p.cu_seqlens[s + 1], p.num_tokens) - p.cu_seqlens[s]); }
+// The keys that a row holds, at most what its table has places for (a length may be anything); negative: idle.
+__device__ __forceinline__ int keys_held(const BlockArgs& p, int row) { return min(p.c.lens[row], p.c.pages_per_row << p.c.page_shift); }
 // The batch entry and the token tile of CTA `index` (of all token tiles of all entries); false: there is none.
 // Tiles are numbered from the one with the most keys down, so the long ones start first: depth = keys in units of a
 // tile's tokens, and for at most 32 entries the number of tiles beyond a depth is one warp sum.
@@ -286,7 +288,7 @@ __device__ __forceinline__ bool find_tile(const BlockArgs& p, int index, int til
         if (lane < p.num_seqs) {
             n = (entry_tokens(p, lane) + tile_tokens - 1) / tile_tokens;
             const int row = p.rows != nullptr ? p.rows[lane] : lane;
-            if (row >= 0 && row < p.c.num_rows) behind = max(0, p.c.lens[row]) / tile_tokens;
+            if (row >= 0 && row < p.c.num_rows) behind = max(0, keys_held(p, row)) / tile_tokens;
         }
         // the largest depth d such that the tiles of depth > d are at most `index`; tile t of an entry has depth behind + t + 1
         const int deepest = __reduce_max_sync(0xffffffffu, n > 0 ? behind + n : 0);
@@ -392,9 +394,10 @@ __global__ void __launch_bounds__(kPrefix ? Geo<D, kBlocks>::kBoundThreads : Geo
                 j.token0 = first + tile * tile_tokens;
                 j.tokens = n - tile * tile_tokens;
                 j.work = first >= 0 && j.tokens > 0;
-                if (row >= 0 && row < p.c.num_rows && p.c.lens[row] >= 0) {
+                const int behind = row >= 0 && row < p.c.num_rows ? keys_held(p, row) : -1;
+                if (behind >= 0) {
                     const long long room = static_cast<long long>(p.c.pages_per_row) << p.c.page_shift;
-                    j.held = p.c.lens[row] + tile * tile_tokens;
+                    j.held = behind + tile * tile_tokens;
                     const long long seen = static_cast<long long>(j.held) + min(j.tokens, tile_tokens);
                     j.total_keys = static_cast<int>(seen < room ? seen : room);
                     j.pages = p.c.page_table + static_cast<size_t>(row) * p.c.pages_per_row;
