@@ -166,10 +166,16 @@ class PagedKVCache:
         K.kv_append_paged_fp8(self, layer, k, v, cu_seqlens, num_tokens, num_seqs, rows, stream)
 
     def gather(self, layer: int, row: int, count: int):
-        """Keys and values 0..count-1 of a row as fp32 [kv heads, count, head dim], for tests and inspection."""
+        """Keys and values 0..count-1 of a row as fp32 [kv heads, count, head dim], for tests and inspection; zeros where the row
+        has no page."""
+        if not (0 <= layer < self.num_layers and 0 <= row < self.num_rows and 0 <= count <= self.pages_per_row * self.page_size):
+            raise RhError("PagedKVCache", 1, f"gather of layer {layer}, row {row}, {count} keys: out of range")
         pages = self.page_table[row, : -(-count // self.page_size)].long()
+        there = (pages >= 0) & (pages < self.num_pages)
+        pages = torch.where(there, pages, torch.zeros_like(pages))
         out = []
         for codes, scale in ((self.k, self.k_scale), (self.v, self.v_scale)):
             x = K.dequantize_kv_fp8(codes[layer, pages].contiguous(), scale[layer, pages])
-            out.append(x.transpose(0, 1).reshape(self.num_kv_heads, -1, self.head_dim)[:, :count])
+            x = torch.where(there[:, None, None, None], x, torch.zeros_like(x))
+            out.append(x.transpose(0, 1).reshape(self.num_kv_heads, pages.numel() * self.page_size, self.head_dim)[:, :count])
         return tuple(out)
