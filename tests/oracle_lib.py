@@ -22,6 +22,11 @@ _p, _i, _f, _l = C.c_void_p, C.c_int, C.c_float, C.c_long
 _sz, _u64, _u32, _i32, _u16, _u8 = C.c_size_t, C.c_uint64, C.c_uint32, C.c_int32, C.c_uint16, C.c_uint8
 
 
+def reference_sources() -> bool:
+    """Whether the reference's sources lie under REFERENCE_ROOT (a checkout's folder may exist and be empty)."""
+    return (REFERENCE_ROOT / "src" / "kernels").is_dir()
+
+
 def _make(target: str) -> None:
     subprocess.run(["make", "-C", str(ORACLE_DIR), f"REF={REFERENCE_ROOT}", target], check=True, capture_output=True)
 
@@ -75,7 +80,7 @@ def load_ref_host():
     """The reference's host helpers; None when neither the prebuilt library nor the reference sources exist."""
     path = ref_host_path()
     if not path.exists():
-        if not REFERENCE_ROOT.exists():
+        if not reference_sources():
             return None
         _make("_ref/libref_host.so")
     lib = C.CDLL(str(path))
@@ -101,7 +106,7 @@ def load_ref_cuda():
     """The reference's CUDA kernels (sm_100a); None when the prebuilt library is absent."""
     path = ref_cuda_path()
     if not path.exists():
-        if not REFERENCE_ROOT.exists():
+        if not reference_sources():
             return None
         _make("_ref/libref_cuda.so")
     lib = C.CDLL(str(path))
@@ -128,7 +133,7 @@ def load_ref_matmul():
     """The reference's W8A8 linear layer (matmul.cu + cuBLASLt); None when the prebuilt library is absent."""
     path = ORACLE_DIR / "_ref" / "libref_matmul.so"
     if not path.exists():
-        if not REFERENCE_ROOT.exists():
+        if not reference_sources():
             return None
         _make("_ref/libref_matmul.so")
     lib = C.CDLL(str(path))
