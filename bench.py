@@ -277,6 +277,11 @@ def run_reference_arm(args, cfg):
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
         return
+    sys.path.insert(0, str(ROOT / "tests"))
+    from oracle_lib import load_ref_host
+    if load_ref_host() is None:          # the oracle port alone is this repository's code, not the reference
+        print(json.dumps({"impl": "reference", "unavailable": "neither the reference's compiled host helpers nor its sources are on this machine"}), flush=True)
+        return
     threads = os.cpu_count() or 1
     _, per_row = step_bytes_per_row(cfg)
     budget = 90.0
