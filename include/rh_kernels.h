@@ -282,7 +282,7 @@ int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
  * num_splits > 1 (long histories in front of few new tokens) deals every row's keys to that many CTAs, whose states are
  * joined from partial_or_null: scratch of rh_flash_prefill_packed_scratch_floats(...) floats, 16-byte aligned, one per call that
  * may overlap in time.  rh_flash_prefill_packed_splits suggests a count (max_keys: the longest row with its new tokens).
- * out, q and the scratch must be 16-byte aligned, q_stride a multiple of 8.  Several entries may name the same row here.  out must
+ * out, q and the scratch must be 16-byte aligned, q_stride a multiple of 8, scale finite.  Several entries may name the same row here.  out must
  * not overlap q.
  * tcgen05 kernel, one CTA per SM holding 256 or all 512 of its tensor-memory columns for its lifetime. */
 int rh_flash_prefill_packed_splits(int num_tokens, int num_seqs, int max_keys, int num_q_heads, int num_kv_heads,
@@ -296,6 +296,7 @@ int rh_flash_prefill_packed_bf16(void* out, const void* q, long long q_stride, c
  * j = 0 .. lens[row of b] of its row (as rh_flash_decode_split_bf16: the new token's key sits at lens[row], appended
  * before this call).  out [num_seqs][num_q_heads][head_dim] bf16; q the same with q_stride elements between entries.
  * An entry whose row is idle, or that sees no key, gets zeros, whatever its q holds.  Several entries may name the same row here.
+ * scale must be finite.
  *
  * shared_pages / shared_len (both or neither; device memory): the first *shared_len keys of every active entry lie in
  * the pages shared_pages[0 .. pages_per_row - 1] (e.g. the page-table row of any entry after rh_kv_pages_fork), and

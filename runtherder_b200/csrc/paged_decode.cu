@@ -625,6 +625,7 @@ extern "C" int rh_flash_decode_paged_bf16(void* out, const void* q, long long q_
                "%s: num_seqs * pages_per_row * page_size must stay below 2^35", fn);
     RH_REQUIRE(num_q_heads >= 1 && num_q_heads % cache->num_kv_heads == 0, RH_ERR_INVALID_ARG, "%s: num_q_heads must be a multiple of num_kv_heads", fn);
     RH_REQUIRE(num_q_heads <= 1024, RH_ERR_UNSUPPORTED_DIM, "%s: at most 1024 query heads", fn);
+    RH_REQUIRE(std::isfinite(scale * paged::kLog2e), RH_ERR_INVALID_ARG, "%s: scale must be finite (and so must scale * log2 e)", fn);
     RH_REQUIRE(q_stride >= static_cast<long long>(num_q_heads) * cache->head_dim, RH_ERR_INVALID_ARG, "%s: q_stride is below num_q_heads * head_dim", fn);
     RH_REQUIRE(host::aligned16(q) && q_stride % 8 == 0 && host::aligned16(partial), RH_ERR_MISALIGNED,
                "%s: q and partial must be 16-byte aligned, q_stride a multiple of 8", fn);

@@ -1150,6 +1150,7 @@ extern "C" int rh_flash_prefill_packed_bf16(void* out, const void* q, long long 
     RH_REQUIRE(rows_or_null != nullptr || num_seqs <= cache->num_rows, RH_ERR_INVALID_ARG, "%s: more sequences than table rows", fn);
     RH_REQUIRE(num_q_heads >= 1 && num_q_heads % cache->num_kv_heads == 0, RH_ERR_INVALID_ARG, "%s: num_q_heads must be a multiple of num_kv_heads", fn);
     RH_REQUIRE(num_q_heads <= 1024, RH_ERR_UNSUPPORTED_DIM, "%s: at most 1024 query heads", fn);
+    RH_REQUIRE(std::isfinite(scale * paged::kLog2e), RH_ERR_INVALID_ARG, "%s: scale must be finite (and so must scale * log2 e)", fn);
     RH_REQUIRE(num_splits >= 1 && num_splits <= 64, RH_ERR_INVALID_ARG, "%s: num_splits must be in 1..64", fn);
     RH_REQUIRE(num_splits == 1 || partial_or_null != nullptr, RH_ERR_INVALID_ARG, "%s: splits need scratch", fn);
     RH_REQUIRE(q_stride >= static_cast<long long>(num_q_heads) * cache->head_dim, RH_ERR_INVALID_ARG, "%s: q_stride is below num_q_heads * head_dim", fn);

@@ -5,7 +5,7 @@ import torch
 
 from runtherder_b200._lib import RhError
 from runtherder_b200.kv_cache import PagedKVCache
-from test_paged_refusals import A, DIM, append, decode, pages, prefill, refused, slabs
+from test_paged_refusals import A, DIM, INVALID, append, decode, pages, prefill, refused, slabs
 
 
 @pytest.mark.parametrize("rows", [(1 << 24) + 1, 1 << 27, 1 << 28, 715827883, (1 << 30) - 1])
@@ -20,6 +20,14 @@ def test_more_rows_than_the_page_operations_can_number(rows):
     refused(DIM, "rh_kv_pages_compact", c, None)
     refused(DIM, *decode(c))
     refused(DIM, *prefill(c))
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38])
+def test_softmax_scales_that_are_no_numbers(scale):
+    """The prefill would take a NaN for the smallest scale there is, and weigh all keys alike."""
+    c = pages()
+    refused(INVALID, "rh_flash_decode_paged_bf16", A, A, 512, c, 0, None, 2, 4, scale, A, None, None, None)
+    refused(INVALID, "rh_flash_prefill_packed_bf16", A, A, 512, c, 0, None, A, 4, 2, 4, scale, A, 2, None)
 
 
 def test_the_class_refuses_them_too():
