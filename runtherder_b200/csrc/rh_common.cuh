@@ -197,13 +197,13 @@ __device__ __forceinline__ uint2 pack_e4m3x8(const float (&y)[8], float inv) {
     return make_uint2(w[0], w[1]);
 }
 
-// ---- correctly rounded divisions without the division subroutine ------------------------------
+// ---- correctly rounded divisions in a few fused multiply-adds ------------------------------
 //
 // The reference computes scale = amax / qmax and inv = qmax / amax with IEEE division, and the
-// sigmoid as 1.0f / (1.0f + e).  nvcc's division is a reciprocal approximation, refinement steps,
-// a range check and a branch to a slow path.  The sequences below give the same correctly rounded
-// results for the operand ranges that occur (amax is a bf16 value, qmax is 127 or 448; d = 1 + e >= 1)
-// — rh_selftest() proves it exhaustively on the device it runs on — and fall back to `/` outside.
+// sigmoid as 1.0f / (1.0f + e).  The sequences below form a quotient from an approximate reciprocal and correct it
+// by its exact remainder, one fused multiply-add each (Markstein, IBM J. Res. Dev. 34, 1990), the reciprocal by
+// Newton's iteration; they give the same correctly rounded results as `/` for the operand ranges that occur (amax
+// is a bf16 value, qmax is 127 or 448; d = 1 + e >= 1) — rh_selftest() proves it exhaustively on the device it runs on — and fall back to `/` outside.
 
 __device__ __forceinline__ float rcp_approx(float x) {
     float r;
@@ -229,7 +229,7 @@ __device__ __forceinline__ float quant_scale(float amax) {       // amax / kQMax
     if (amax >= 1.0e-30f && amax <= 1.0e30f) return div_refine(amax, qmax, 1.0f / qmax);
     return amax / qmax;
 }
-// sigmoid of two gates, s = 1 / (1 + e), e = __expf(-g) = ex2.approx.ftz(-g * log2(e)), with the
+// sigmoid of two gates, s = 1 / (1 + e), e = 2^(-g log2 e) by ex2.approx (rh_selftest holds it against __expf), with the
 // reciprocal refined kSteps times.  Valid for g >= kGateExactBelow (1 + e stays far below the range
 // where its reciprocal turns subnormal); callers send smaller gates down the IEEE-division path.
 constexpr float kGateExactBelow = -85.0f;
