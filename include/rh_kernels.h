@@ -214,6 +214,13 @@ int rh_bias_rope_kv_fp8(void* q, void* k_out_or_null, const void* k_in, const vo
  * attention; advance.  Rows, lengths and pages are checked where they are used: a token of an idle or unknown row,
  * or one whose page is missing (-1) or no page of the pool, is not stored, and such a page's keys are not attended.
  *
+ * Accuracy.  The append stores what rh_quantize_kv_fp8 does, bit for bit.  The attention kernels are held to exact attention
+ * over the values in the pages within the bf16 rounding of the result plus, relative to A = sum_j p_j |v_j|: 2^-11 for the
+ * weights, which enter the second product as f16; in the tcgen05 forms (packed prefill, prefix of 17 or more query rows per kv
+ * head) twice 2^-11 more for V (its scale and the product with it are rounded to f16), and scores that come from q within 2^-16 of
+ * its row's largest value.  Weights below 2^-32 of a row's largest (times 2^8 v_scale beside keys with a V scale above 1/2) are lost.
+ * That is more than the one-sequence kernels allow themselves: they are within one bf16 ulp.
+ *
  * `scratch` serves the page operations (reserve, fork, compact); calls on one cache that may overlap in time (two
  * streams, two graphs) must be ordered by the caller.  The struct is read during the call only. */
 typedef struct rh_kv_pages {
@@ -272,7 +279,8 @@ int rh_kv_pages_fork(const rh_kv_pages* cache, const int* parents, const int* ch
 int rh_kv_pages_copy(const rh_kv_pages* cache, const int* src, const int* dst, int count, void* stream);
 
 /* Packs the used pages to the front of the pool, all layers: the k-th used page at or above the number of used
- * pages moves to the k-th free page below it, and the page table and the counts follow. */
+ * pages moves to the k-th free page below it, and the page table and the counts follow.  Copies of page ids that the caller keeps
+ * elsewhere (shared_pages that are not a row of the table) do not. */
 int rh_kv_pages_compact(const rh_kv_pages* cache, void* stream);
 
 /* Causal attention of a packed batch's new tokens: token i of an entry attends keys 0 .. lens[row] + i of its row
@@ -300,7 +308,7 @@ int rh_flash_prefill_packed_bf16(void* out, const void* q, long long q_stride, c
  *
  * shared_pages / shared_len (both or neither; device memory): the first *shared_len keys of every active entry lie in
  * the pages shared_pages[0 .. pages_per_row - 1] (e.g. the page-table row of any entry after rh_kv_pages_fork), and
- * these are read once for all entries.  An entry that holds fewer keys attends those it holds.  The entries' own
+ * these are read once for all entries; a row that is named so must keep its pages.  An entry that holds fewer keys attends those it holds.  The entries' own
  * table rows list the shared pages too; what is shared beyond a multiple of 256 keys is read through them.
  *
  * partial: caller-owned scratch of rh_flash_decode_paged_scratch_floats(...) floats, 16-byte aligned like q (out: 8-byte);

@@ -340,7 +340,9 @@ __global__ void __launch_bounds__(256) advance_kernel(const Tables t, const int*
 
 // Bookkeeping is one CTA's work: its steps depend on one another and their data are a few kilobytes, so it is bound by the
 // latency of some ten rounds of loads and barriers (a fork of 8 children 9.5 us with its copies, 13 us for the bookkeeping
-// of 64 children with 31 shared pages each).
+// of 64 children with 31 shared pages each; a reserve in which nothing is lacking 3.3 us, an advance of 32 rows 1.5).  The search for
+// free pages starts at page 0 and takes 4096 pages a step: a reserve of 32 rows that each need a page, 95 % of the pool used, 5.0 us
+// with 1500 pages, 8.8 with 20 000, 46 with 200 000.
 //
 // children[i] becomes a second owner of parents[i]'s whole pages and of a page of its own for the keys behind them.
 // All parents are read before any child is written (a beam step permutes rows), and the pages of the children's old
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs p) {
     const long long items = static_cast<long long>(n) * p.num_layers * 2 * chunks;
     for (long long item = blockIdx.x; item < items; item += gridDim.x) {
         int chunk, slab, layer, m;
-        if (items <= INT_MAX) {                                    // (64-bit divisions are calls of some 70 instructions each)
+        if (items <= INT_MAX) {                                    // (a 64-bit division is a call)
             const unsigned rest = static_cast<unsigned>(item) / static_cast<unsigned>(chunks), block = rest >> 1;
             chunk = static_cast<int>(static_cast<unsigned>(item) - rest * static_cast<unsigned>(chunks));
             slab = static_cast<int>(rest & 1u);

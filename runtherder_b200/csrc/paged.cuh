@@ -69,7 +69,7 @@ __device__ __forceinline__ bool named_before(const int* rows, int s, int row) {
 
 namespace host {
 
-// Checks a cache description (all the arrays that `needs_tables` calls use included) and reports through fail().
+// Checks a cache description, all of its arrays whatever the call uses, and reports through fail().
 int check_pages(const rh_kv_pages* c, const char* fn);
 // The same plus the layer index; fills `out` with that layer.
 int paged_layer(const rh_kv_pages* c, int layer, const char* fn, paged::Layer* out);

@@ -22,7 +22,8 @@
 // warp's own ring, a tile ahead, the scales come by one asynchronous copy per lane; there is no barrier among warps.
 //
 // Measured (B200, 32/8 heads of 128): 8 x 32768 keys 68 us = 5.3 TB/s, 64 x 2000 keys 38.8 us = 3.8 TB/s, of 6.5 for a copy; a
-// lone sequence of 8196 keys (24/8 heads) 14 us.  The decode kernel alone on 64 x 2000 keys takes 34 us (DRAM 56 % busy, issue slots
+// lone sequence of 8196 keys (24/8 heads) 14 us out of L2, 17 us with 28 caches in turn (flash_decode.cu, which joins four warps in a CTA before it
+// writes a state, 9.3 - 9.8 us so; 65536 keys 35 us in either).  The decode kernel alone on 64 x 2000 keys takes 34 us (DRAM 56 % busy, issue slots
 // 46 %, 385 instructions per tile): a warp's tile is a chain of some 2000 cycles (wait, products, exponentials, transposes, products),
 // sixteen warps of 128 registers fill an SM (twenty of 96 spill: 64 x 2000 keys 44.9 us), and the E4M3 conversions alone are 8 us at one per
 // cycle and SM.  What a small call waits for is latency:
@@ -55,7 +56,9 @@ constexpr int kStages = 2;             // tiles in a warp's ring (with three, 8 
 static_assert((kStages & (kStages - 1)) == 0, "counters wrap");
 constexpr int kDecCtas = 4;            // CTAs per SM
 constexpr float kLag = 8.0f;           // how far (log2) the running maximum may lie below the true one
-constexpr float kShift = 7.0f;         // weights enter the second product as 2^7 * weight (at most 2^15): small ones stay normal in f16
+// Weights enter the second product as 2^7 * weight (at most 2^15), rounded to f16 once: 2^-11 each, an eighth of the bf16 store's rounding, and
+// below 2^-32 of the row's largest lost.  (flash_decode.cu enters two f16 parts of each.)
+constexpr float kShift = 7.0f;
 
 // D(16x8, fp32) += A(16x16, f16, row) * B(16x8, f16, col)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -23,20 +23,24 @@
 //     above 2^-9 of it is exact, smaller ones are off by at most 2^-16 of it.  Two E4M3 products take the time of one f16
 //     product, and nothing has to convert K: clock stamps of the f16 form (0.80 ms on 8192 tokens, 32/8 heads of 128) had
 //     every product waiting for the converted K tile, and both row blocks in step behind it.
-// (2) The V scale is folded into the f16 V operand (one rounding of 2^-11, like a weight's) instead of riding in the
-//     exponent: no per-key additions and multiplications in the softmax.  f16 holds vs * 448 only for vs in 2^-22 .. 2^-1
-//     (with a common factor of 2^8); a tile with a scale outside keeps the exponent form, and both add up in one O.
+// (2) The V scale is folded into the f16 V operand instead of riding in the exponent: no per-key additions and multiplications
+//     in the softmax.  That is two roundings of 2^-11, the scale's (common to a key's row of V) and the product's; flash_prefill_ws.cu
+//     has neither.  f16 holds vs * 448 only for vs in 2^-22 .. 2^-1 (with a common factor of 2^8); a tile with a scale outside
+//     keeps the exponent form, and both add up in one O: beside a key of scale vs > 1/2 the others' weights are taken relative to a
+//     maximum up to 2^8 vs higher, and f16 loses what is below 2^-32 of that.
 // (3) The running maximum may lag the true one by up to 2^8, so that O is rescaled a handful of times per row instead of on most
 //     tiles.  Weights carry a factor of 2^7: they stay below 2^15, and what f16 loses of small ones is below 2^-32 of the largest
 //     (unshifted it was 2^-25: over 8192 keys that may be 2^-12 of the output, over 128k keys 2^-8, all of it missing from the
 //     numerator and present in the denominator).  Each weight is rounded to f16 once, 2^-11; the denominator sums the unrounded
-//     fp32 weights.
+//     fp32 weights, so a row that one key dominates is off by up to 2^-11 (its largest weight is seldom a power of two; in
+//     flash_prefill_ws.cu it is exactly 1): an eighth of the bf16 store's 2^-8, like every other rounding here.
 // (4) Rows carry their own last visible key, pages may be missing, and places that no row may see may hold anything: the
 //     tiles that reach past some row's last key (and only those) replace NaN codes of V by zero and mark the key, so that
 //     exactly the rows that see it get NaN.
 //
-// Measured (B200, 32/8 heads of 128).  One prompt of 8192 tokens 615 us = 890 TFLOP/s at full clocks (flash_prefill_ws.cu on a contiguous
-// cache: 718 us); six ragged prompts of 8192 tokens together 228 us = 634 TFLOP/s; the 32768 shared keys of 128 sequences about 85 us.
+// Measured (B200, 32/8 heads of 128).  Six ragged prompts of 8192 tokens together 228 us = 634 TFLOP/s; one prompt of 8192 tokens 610 - 665
+// us = 825 - 900 TFLOP/s, by how long the power cap leaves the clock up (flash_prefill_ws.cu on a contiguous cache: 718 us); the 32768
+// shared keys of 128 sequences about 85 us.
 // A tile of 64 keys takes two row blocks 1.3 us and costs 1152 cycles of products (tensor pipe 30 - 39 % busy) and 1024 of
 // exponentials; issue slots are 53 % busy.  What bounds it is the chain of a tile through a softmax warp (scores from tensor memory,
 // maximum, exponentials, weights to tensor memory, the product that frees them).  Tried without gain: 128-key tiles (765 us), the next
@@ -1130,7 +1134,7 @@ extern "C" int rh_flash_prefill_packed_splits(int num_tokens, int num_seqs, int 
             best = s;
         }
     }
-    (void)head_dim;
+    (void)head_dim;      // (the units are a tile's and a CTA's times, whose ratio was fitted for heads of 128 and used for 64 too)
     return best;
 }
 
