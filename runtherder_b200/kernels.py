@@ -274,6 +274,8 @@ def _token_rows(cache, t, num_tokens: int, heads: int, head_dim: int, name: str)
     if t.is_contiguous():
         if t.numel() < num_tokens * width:
             raise RhError(name, 1, f"{name} holds {t.numel()} elements, {num_tokens * width} needed")
+        if num_tokens > 1 and t.dim() == 3 and t.shape[0] >= num_tokens and t.shape[2] == head_dim and t.shape[1] != heads:
+            raise RhError(name, 1, f"{name} has {t.shape[1]} heads per token, {heads} expected: pass the slice of them")
         return t.data_ptr(), width
     inside = (head_dim, 1) if t.dim() == 3 else (1,)
     if t.dim() not in (2, 3) or t.shape[0] < num_tokens or t.stride()[1:] != inside or t.shape[1:].numel() != width or \
