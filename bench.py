@@ -267,7 +267,7 @@ def cpu_baseline(cfg, seconds: float):
                               "sample": f"{one_rows} rows on one thread"},
             "sample": f"{rows} of {cfg.tokens} token rows of the same four ops, row-parallel over {threads} host "
                       f"threads; {'reference test helpers (double precision) for norm, RoPE, FP8 KV, SwiGLU; ' if kind == 'reference' else ''}"
-                      f"oracle port for INT8 quantisation and the gather (the reference has no host code for them); "
+                      f"{'oracle port for INT8 quantisation and the gather (the reference has no host code for them); ' if kind == 'reference' else 'oracle port for all of it; '}"
                       f"{'RoPE through the plain-theta table its host helper builds (no llama3 rescaling), ' if kind == 'reference' else ''}"
                       f"gather from a 4096-row window of the table"}
 
