@@ -1134,7 +1134,7 @@ extern "C" int rh_flash_prefill_packed_splits(int num_tokens, int num_seqs, int 
             best = s;
         }
     }
-    (void)head_dim;      // (the units are a tile's and a CTA's times, whose ratio was fitted for heads of 128 and used for 64 too)
+    (void)head_dim;      // (one ratio of a CTA's time to a tile's serves both sizes of head)
     return best;
 }
 

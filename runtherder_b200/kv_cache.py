@@ -103,6 +103,11 @@ class PagedKVCache:
         self._adopt(**slabs)
         return self
 
+    def __setattr__(self, name, value) -> None:
+        if name in self.SLABS + ("scratch",) and "_struct" in self.__dict__:     # the kernels have the addresses of those it was made of
+            raise RhError("PagedKVCache", 1, f"{name} of a cache cannot be replaced: copy into it, or make a cache by from_tensors")
+        super().__setattr__(name, value)
+
     def _adopt(self, **slabs) -> None:
         if set(slabs) != set(self.SLABS):
             raise RhError("PagedKVCache", 1, f"PagedKVCache is made of {', '.join(self.SLABS)}")

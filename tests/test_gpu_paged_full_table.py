@@ -14,9 +14,8 @@ pytestmark = pytest.mark.gpu
 def full(rows, per, ps, heads, dim, seed):
     """Rows whose every place has a page of numbers of its own."""
     c = filled([per * ps - 1] * rows, heads=heads, dim=dim, ps=ps, seed=seed, stale_nan=False)
-    c.page_table = c.page_table[:, :per].contiguous()
     from runtherder_b200.kv_cache import PagedKVCache
-    return PagedKVCache.from_tensors(**{n: getattr(c, n) for n in PagedKVCache.SLABS})
+    return PagedKVCache.from_tensors(**{**{n: getattr(c, n) for n in PagedKVCache.SLABS}, "page_table": c.page_table[:, :per].contiguous()})
 
 
 @pytest.mark.parametrize("dim,ps,hq,hkv", [(128, 16, 12, 4), (64, 64, 8, 1)])
